@@ -328,7 +328,7 @@ def work(case):
 def _exact_rope(s):
     tokens, heads, dim = s["qkv"].shape[0], s["n_heads"], s["dim"]
     out = s["qkv"].double()
-    x = out[:, :heads * dim].reshape(tokens, heads, 2, dim // 2)
+    x = out[:, :heads * dim].clone().reshape(tokens, heads, 2, dim // 2)
     for i in range(dim // 2):
         angle = s["positions"][int(s["axis"][i])].double() * math.exp(-math.log(_THETA) * 2 * i / dim)
         turn = torch.polar(torch.ones_like(angle), -angle if s["inverse"] else angle)[:, None]
