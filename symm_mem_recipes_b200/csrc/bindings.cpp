@@ -9,6 +9,7 @@
 #include <cuda_runtime_api.h>
 #include <torch/extension.h>
 
+#include <math.h>
 #include <stdlib.h>
 #include <string.h>
 
@@ -16,6 +17,7 @@
 #include <memory>
 #include <atomic>
 #include <mutex>
+#include <stdexcept>
 #include <thread>
 
 #include "kernels/decode_stack.h"
@@ -321,6 +323,90 @@ c10::optional<torch::Tensor> matmul_local(const torch::Tensor& a, const torch::T
   if (trace.has_value()) args.trace = trace_words(*trace, dev, args.num_sms);
   rt_check(launch_ag_matmul_2cta(args, stream), "matmul");
   return c;
+}
+
+// ---- 4-bit KV cache and rotation by several axes: checks of arguments ----
+// A refused argument raises SymmMemError in Python.  Shapes and types are looked at before devices, so that every refusal
+// can be seen without a GPU.
+struct Refusal : std::runtime_error {
+  using std::runtime_error::runtime_error;
+};
+template <typename... T>
+void need(bool ok, const T&... what) {
+  if (!ok) throw Refusal(c10::str(what...));
+}
+void need_on_gpu(const torch::Tensor& t, int device, const char* name) {
+  need(t.is_cuda() && (device < 0 || t.get_device() == device), name, " must be on ", device < 0 ? "a" : "the cache's", " GPU");
+}
+bool aligned16(const torch::Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; }
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  auto end = [](const torch::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += t.size(i) > 0 ? (t.size(i) - 1) * t.stride(i) : 0;
+    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+  };
+  return a.numel() > 0 && b.numel() > 0 && a.data_ptr() < end(b) && b.data_ptr() < end(a);
+}
+
+// The cache's tensors as the kernels take them; `batch` comes back from their shape.
+Kv4Cache kv4_cache(const torch::Tensor& kc, const torch::Tensor& ks, const torch::Tensor& vc, const torch::Tensor& vs,
+                   const c10::optional<torch::Tensor>& weights, int64_t max_seq, int64_t* batch) {
+  need(kc.dim() == 4 && kc.scalar_type() == torch::kUInt8 && (kc.size(3) == 32 || kc.size(3) == 64),
+       "k_codes must be uint8 [batch, kv heads, slots, head_dim / 2] with a head_dim of 64 or 128");
+  const int64_t D = 2 * kc.size(3), slots = kc.size(2);
+  need(vc.sizes() == kc.sizes() && vc.scalar_type() == torch::kUInt8, "v_codes must be like k_codes");
+  for (const torch::Tensor* s : {&ks, &vs})
+    need(s->dim() == 4 && s->scalar_type() == torch::kBFloat16 && s->size(0) == kc.size(0) && s->size(1) == kc.size(1) &&
+         s->size(2) == slots && s->size(3) == D / 32, "scales must be bfloat16 [batch, kv heads, slots, head_dim / 32]");
+  need(slots % 64 == 0, "a cache has a multiple of 64 slots");
+  need(max_seq >= 0 && max_seq <= slots, "max_seq must be at most the cache's ", slots, " slots");
+  need(kc.numel() == 0 || kc.size(0) * kc.size(1) * (slots / 64) < (1ll << 30), "the cache has too many tiles");
+  need(kc.is_contiguous() && vc.is_contiguous() && ks.is_contiguous() && vs.is_contiguous(), "a cache's tensors must be contiguous");
+  need(aligned16(kc) && aligned16(vc) && aligned16(ks) && aligned16(vs), "a cache's tensors must start on 16 bytes");
+  if (weights.has_value()) {
+    need(weights->dim() == 3 && weights->scalar_type() == torch::kFloat32 && weights->is_contiguous() &&
+         weights->size(0) == kc.size(0) && weights->size(1) == kc.size(1) && weights->size(2) == slots && aligned16(*weights),
+         "weights must be contiguous float32 [batch, kv heads, slots]");
+  }
+  need(!overlap(kc, vc) && !overlap(ks, vs), "keys and values must not share memory");
+  need_on_gpu(kc, -1, "k_codes");
+  const int dev = kc.get_device();
+  need_on_gpu(vc, dev, "v_codes");
+  need_on_gpu(ks, dev, "k_scales");
+  need_on_gpu(vs, dev, "v_scales");
+  if (weights.has_value()) need_on_gpu(*weights, dev, "weights");
+  *batch = kc.size(0);
+  Kv4Cache c{};
+  c.k_codes = static_cast<uint8_t*>(kc.data_ptr());
+  c.v_codes = static_cast<uint8_t*>(vc.data_ptr());
+  c.k_scales = ks.data_ptr();
+  c.v_scales = vs.data_ptr();
+  c.weights = weights ? static_cast<float*>(weights->data_ptr()) : nullptr;
+  c.hkv = (int)kc.size(1);
+  c.slots = (int)slots;
+  c.head_dim = (int)D;
+  c.max_seq = (int)max_seq;
+  return c;
+}
+void need_per_sequence(const c10::optional<torch::Tensor>& t, int64_t batch, const char* name) {
+  need(!t.has_value() || (t->dim() == 1 && t->size(0) == batch && t->scalar_type() == torch::kInt32 && t->is_contiguous()), name,
+       " must be an int32 tensor of one element a sequence");
+}
+const int* int_ptr(const c10::optional<torch::Tensor>& t) { return t ? static_cast<const int*>(t->data_ptr()) : nullptr; }
+
+// Frequencies of the pairs in units of 2^-64 turns; computed when theta or head_dim is another than in the last call.
+const uint64_t* rope_frequencies(double theta, int64_t head_dim) {
+  thread_local double last_theta = 0.0;
+  thread_local int64_t last_dim = 0;
+  thread_local uint64_t table[64];
+  if (theta != last_theta || head_dim != last_dim) {
+    constexpr long double kTwoPi = 6.283185307179586476925286766559L;
+    for (int64_t i = 0; i < head_dim / 2; ++i)
+      table[i] = (uint64_t)roundl(ldexpl(powl((long double)theta, -2.0L * i / head_dim) / kTwoPi, 64));
+    last_theta = theta;
+    last_dim = head_dim;
+  }
+  return table;
 }
 
 }  // namespace
@@ -1111,6 +1197,187 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return y;
   }, py::arg("x"), py::arg("tensors"), py::arg("pos0"), py::arg("pos"), py::arg("hq"), py::arg("eps"),
      py::arg("rope_theta"), py::arg("timeout_ns"));
+
+  // ---- rotation by positions of several axes, 4-bit KV cache ----
+  py::register_exception_translator([](std::exception_ptr p) {
+    try {
+      if (p) std::rethrow_exception(p);
+    } catch (const Refusal& e) {
+      PyErr_SetString(py::module_::import("symm_mem_recipes_b200.errors").attr("SymmMemError").ptr(), e.what());
+    }
+  });
+  m.def("rope_axes", [](const torch::Tensor& qkv, int64_t n_heads, int64_t D, const torch::Tensor& positions,
+                        const std::vector<int64_t>& sections, double theta, bool interleaved, bool inverse) {
+    need(qkv.dim() == 2 && qkv.scalar_type() == torch::kBFloat16, "qkv must be a 2-D bfloat16 tensor");
+    need(D == 64 || D == 128, "head_dim must be 64 or 128");
+    need(n_heads >= 0 && n_heads <= qkv.size(1) / D, "need n_heads * head_dim <= row length");
+    need(theta > 1.0 && theta < 1e18, "theta must be larger than 1");
+    const int64_t axes = (int64_t)sections.size(), T = qkv.size(0);
+    need(axes >= 1 && axes <= 16, "need one to 16 sections");
+    int64_t pairs = 0;
+    for (int64_t share : sections) {
+      need(share >= 0 && share <= 64, "a section is a number of pairs");
+      pairs += share;
+    }
+    need(pairs == D / 2, "the sections must add up to the ", D / 2, " pairs of a head");
+    need(positions.scalar_type() == torch::kInt32 &&
+         ((positions.dim() == 2 && positions.size(0) == axes && positions.size(1) == T) ||
+          (positions.dim() == 1 && axes == 1 && positions.size(0) == T)), "positions must be int32 [axes, tokens]");
+    need(T == 0 || positions.stride(-1) == 1 || positions.size(-1) <= 1, "positions must be contiguous along the tokens");
+    need(T <= 1 || qkv.stride(0) >= n_heads * D, "qkv's rows must not overlap");
+    need((qkv.size(1) <= 1 || qkv.stride(1) == 1) && (T <= 1 || qkv.stride(0) % 8 == 0) && aligned16(qkv),
+         "qkv's rows must be contiguous and start on 16 bytes");
+    need_on_gpu(qkv, -1, "qkv");
+    const int dev = qkv.get_device();
+    need(positions.is_cuda() && positions.get_device() == dev, "positions must be on qkv's GPU");
+    RopeAxesArgs a;
+    a.qkv = qkv.data_ptr();
+    a.tokens = T;
+    a.row_stride = qkv.stride(0);
+    a.n_heads = (int)n_heads;
+    a.head_dim = (int)D;
+    a.positions = static_cast<const int*>(positions.data_ptr());
+    a.position_stride = positions.dim() == 2 ? positions.stride(0) : 0;
+    a.inverse = inverse;
+    memcpy(a.frequency, rope_frequencies(theta, D), sizeof(a.frequency));
+    memset(a.axis, 0, sizeof(a.axis));
+    int64_t i = 0;
+    if (interleaved) {      // dealt to the axes in turn until an axis has its share
+      for (int64_t round = 0; i < pairs; ++round)
+        for (int64_t x = 0; x < axes; ++x)
+          if (round < sections[x]) a.axis[i++] = (uint8_t)x;
+    } else {
+      for (int64_t x = 0; x < axes; ++x)
+        for (int64_t k = 0; k < sections[x]; ++k) a.axis[i++] = (uint8_t)x;
+    }
+    c10::cuda::CUDAGuard guard(dev);
+    rt_check(launch_rope_axes(a, current_stream(dev)), "rope_axes");
+  }, py::arg("qkv"), py::arg("n_heads"), py::arg("head_dim"), py::arg("positions"), py::arg("sections"), py::arg("theta"),
+     py::arg("interleaved"), py::arg("inverse"));
+  m.def("kv4_check", [](const torch::Tensor& kc, const torch::Tensor& ks, const torch::Tensor& vc, const torch::Tensor& vs,
+                        const c10::optional<torch::Tensor>& weights, int64_t max_seq) {
+    int64_t batch;
+    kv4_cache(kc, ks, vc, vs, weights, max_seq, &batch);
+  }, py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("weights"), py::arg("max_seq"));
+  m.def("kv4_append", [](const torch::Tensor& k, const torch::Tensor& v, const torch::Tensor& kc, const torch::Tensor& ks,
+                         const torch::Tensor& vc, const torch::Tensor& vs, const c10::optional<torch::Tensor>& weights,
+                         int64_t max_seq, int64_t start0, const c10::optional<torch::Tensor>& start,
+                         const c10::optional<torch::Tensor>& counts) {
+    need(k.dim() == 4 && kc.dim() == 4 && k.sizes() == v.sizes() && k.size(0) == kc.size(0) && k.size(2) == kc.size(1) &&
+         k.size(3) == 2 * kc.size(3), "k and v must be [batch, tokens, kv heads, head_dim] of the cache's sizes");
+    Kv4AppendArgs a{};
+    const torch::Tensor* in[2] = {&k, &v};
+    for (int i = 0; i < 2; ++i) {
+      const torch::Tensor& t = *in[i];
+      need(t.scalar_type() == torch::kBFloat16, "k and v must be bfloat16");
+      bool ok = t.stride(3) == 1 && aligned16(t);
+      for (int j = 0; j < 3; ++j) {
+        ok = ok && (t.size(j) <= 1 || t.stride(j) % 8 == 0);
+        (i ? a.v_stride : a.k_stride)[j] = t.size(j) <= 1 ? 0 : t.stride(j);
+      }
+      need(ok || t.numel() == 0, "the rows of k and v must be contiguous and start on 16 bytes");
+    }
+    need_per_sequence(start, k.size(0), "start");
+    need_per_sequence(counts, k.size(0), "counts");
+    need(start.has_value() || (start0 >= 0 && start0 + k.size(1) <= max_seq), "slots [", start0, ", ", start0 + k.size(1),
+         ") are outside the cache of ", max_seq);
+    int64_t batch;
+    a.cache = kv4_cache(kc, ks, vc, vs, weights, max_seq, &batch);
+    const int dev = kc.get_device();
+    need_on_gpu(k, dev, "k");
+    need_on_gpu(v, dev, "v");
+    if (start.has_value()) need_on_gpu(*start, dev, "start");
+    if (counts.has_value()) need_on_gpu(*counts, dev, "counts");
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.batch = (int)batch;
+    a.tokens = (int)k.size(1);
+    a.start = (int)start0;
+    a.start_dev = int_ptr(start);
+    a.counts = int_ptr(counts);
+    c10::cuda::CUDAGuard guard(dev);
+    rt_check(launch_kv4_append(a, current_stream(dev)), "kv4_append");
+  }, py::arg("k"), py::arg("v"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"),
+     py::arg("weights"), py::arg("max_seq"), py::arg("start0"), py::arg("start"), py::arg("counts"));
+  m.def("kv4_read", [](const torch::Tensor& kc, const torch::Tensor& ks, const torch::Tensor& vc, const torch::Tensor& vs,
+                       int64_t max_seq, int64_t n) {
+    need(n >= 0 && n <= max_seq, "cannot read ", n, " slots of a cache of ", max_seq);
+    int64_t batch;
+    const Kv4Cache cache = kv4_cache(kc, ks, vc, vs, c10::nullopt, max_seq, &batch);
+    const int dev = kc.get_device();
+    c10::cuda::CUDAGuard guard(dev);
+    torch::Tensor k = new_tensor({batch, n, cache.hkv, cache.head_dim}, torch::kBFloat16, dev);
+    torch::Tensor v = new_tensor({batch, n, cache.hkv, cache.head_dim}, torch::kBFloat16, dev);
+    rt_check(launch_kv4_read(cache, (int)batch, (int)n, k.data_ptr(), v.data_ptr(), current_stream(dev)), "kv4_read");
+    return std::make_pair(k, v);
+  }, py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("max_seq"), py::arg("n"));
+  m.def("kv4_decode_attention", [](const torch::Tensor& qkv, const torch::Tensor& kc, const torch::Tensor& ks,
+                                   const torch::Tensor& vc, const torch::Tensor& vs, const c10::optional<torch::Tensor>& weights,
+                                   int64_t max_seq, int64_t hq, int64_t length, const c10::optional<torch::Tensor>& lengths,
+                                   const c10::optional<torch::Tensor>& out) {
+    need(qkv.dim() == 2 && kc.dim() == 4 && qkv.scalar_type() == torch::kBFloat16, "qkv must be a 2-D bfloat16 tensor");
+    const int64_t hkv = kc.size(1), D = 2 * kc.size(3), B = kc.size(0);
+    need(hkv >= 1 && hq >= 1 && hq % hkv == 0 && hq / hkv <= 8, "need hq a multiple of the kv heads with hq / hkv <= 8");
+    need(qkv.size(0) == B && qkv.size(1) == (hq + 2 * hkv) * D, "need qkv [batch, (hq + 2 hkv) * head_dim] of the cache's sizes");
+    need(qkv.stride(1) == 1 && (B <= 1 || qkv.stride(0) % 8 == 0) && aligned16(qkv),
+         "qkv's rows must be contiguous and start on 16 bytes");
+    need(B <= 1024, "at most 1024 sequences");
+    need_per_sequence(lengths, B, "lengths");
+    need(lengths.has_value() || (length >= 0 && length < max_seq), "length ", length, " outside the cache of ", max_seq, " slots");
+    if (out.has_value()) {
+      need(out->dim() == 2 && out->size(0) == B && out->size(1) == hq * D && out->scalar_type() == torch::kBFloat16 &&
+           out->is_contiguous() && aligned16(*out), "out must be contiguous bfloat16 [batch, hq * head_dim], on 16 bytes");
+      need(!overlap(*out, qkv), "out must not share memory with qkv");
+    }
+    int64_t batch;
+    Kv4AttentionArgs a{};
+    a.cache = kv4_cache(kc, ks, vc, vs, weights, max_seq, &batch);
+    const int dev = kc.get_device();
+    need_on_gpu(qkv, dev, "qkv");
+    if (lengths.has_value()) need_on_gpu(*lengths, dev, "lengths");
+    if (out.has_value()) need_on_gpu(*out, dev, "out");
+    c10::cuda::CUDAGuard guard(dev);
+    torch::Tensor o = out.has_value() ? *out : new_tensor({B, hq * D}, torch::kBFloat16, dev);
+    if (B == 0) return o;
+    a.qkv = qkv.data_ptr();
+    a.qkv_stride = qkv.stride(0);
+    a.out = o.data_ptr();
+    a.batch = (int)B;
+    a.group = (int)(hq / hkv);
+    a.length = (int)length;
+    a.lengths = int_ptr(lengths);
+    a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    torch::Tensor workspace = new_tensor({(int64_t)kv4_attention_workspace_bytes(a.cache, a.batch, a.group, a.num_sms)},
+                                         torch::kUInt8, dev);
+    a.workspace = workspace.data_ptr();
+    rt_check(launch_kv4_attention(a, current_stream(dev)), "kv4_decode_attention");
+    return o;
+  }, py::arg("qkv"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("weights"),
+     py::arg("max_seq"), py::arg("hq"), py::arg("length"), py::arg("lengths"), py::arg("out"));
+  m.def("kv4_evict", [](const torch::Tensor& kc, const torch::Tensor& ks, const torch::Tensor& vc, const torch::Tensor& vs,
+                        const torch::Tensor& weights, int64_t max_seq, const torch::Tensor& lengths, int64_t keep, int64_t recent) {
+    need(keep >= 1 && keep <= max_seq, "keep must be between 1 and the cache's ", max_seq, " slots");
+    need(recent >= 0 && recent <= keep, "recent must be between 0 and keep");
+    need(kc.dim() == 4, "k_codes must be uint8 [batch, kv heads, slots, head_dim / 2]");
+    need_per_sequence(lengths, kc.size(0), "lengths");
+    int64_t batch;
+    Kv4EvictArgs a{};
+    a.cache = kv4_cache(kc, ks, vc, vs, weights, max_seq, &batch);
+    const int dev = kc.get_device();
+    need_on_gpu(lengths, dev, "lengths");
+    c10::cuda::CUDAGuard guard(dev);
+    torch::Tensor new_lengths = new_tensor({batch}, torch::kInt32, dev);
+    torch::Tensor list = new_tensor({batch * a.cache.hkv * keep}, torch::kInt32, dev);
+    a.batch = (int)batch;
+    a.keep = (int)keep;
+    a.recent = (int)recent;
+    a.lengths = static_cast<const int*>(lengths.data_ptr());
+    a.new_lengths = static_cast<int*>(new_lengths.data_ptr());
+    a.list = static_cast<int*>(list.data_ptr());
+    rt_check(launch_kv4_evict(a, current_stream(dev)), "kv4_evict");
+    return new_lengths;
+  }, py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("weights"), py::arg("max_seq"),
+     py::arg("lengths"), py::arg("keep"), py::arg("recent"));
 
   // ---- oracles (CPU tensors) ----
   m.def("oracle_rms_norm_bf16", [](torch::Tensor x, c10::optional<torch::Tensor> residual, torch::Tensor w,

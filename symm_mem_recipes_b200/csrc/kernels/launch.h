@@ -224,4 +224,67 @@ bool prefill_attention_preferred(int batch, int seq, int hq, int hkv, int head_d
 int launch_prefill_attention(const void* qkv, void* out, int batch, int seq, int hq, int hkv, int head_dim,
                              cudaStream_t stream);
 
+// ---- rotary embedding by positions of several axes (rope_axes.cu) ----
+struct RopeAxesArgs {
+  void* qkv;                 // [tokens, row_stride] bf16; heads [0, n_heads) of a row are rotated in place
+  long long tokens, row_stride;
+  int n_heads, head_dim;     // 64 or 128
+  const int* positions;      // [axes][position_stride] int32
+  long long position_stride;
+  bool inverse;              // rotate back
+  uint64_t frequency[64];    // of pair i: theta^(-2 i / head_dim) / (2 pi) in units of 2^-64 turns
+  uint8_t axis[64];          // whose position turns pair i
+};
+int launch_rope_axes(const RopeAxesArgs& args, cudaStream_t stream);
+
+// ---- 4-bit KV cache (kv4.cuh has the format) ----
+struct Kv4Cache {
+  uint8_t* k_codes;          // [batch, hkv, slots, head_dim / 2]
+  uint8_t* v_codes;
+  void* k_scales;            // [batch, hkv, slots, head_dim / 32] bf16
+  void* v_scales;
+  float* weights;            // [batch, hkv, slots] accumulated attention weight, or nullptr
+  int hkv, slots, head_dim;  // slots: a multiple of 64; head_dim 64 or 128
+  int max_seq;               // slots in use at most, <= slots
+};
+// Rows [b, t] of k and v, t < counts[b] (all without counts), into slots start + t; a start outside [0, max_seq)
+// writes nothing, tokens behind max_seq are dropped.
+struct Kv4AppendArgs {
+  Kv4Cache cache;
+  const void* k;             // [batch, tokens, hkv, head_dim] bf16, strides in elements, rows 16-byte aligned
+  const void* v;
+  long long k_stride[3], v_stride[3];
+  int batch, tokens;
+  int start;                 // where `start_dev` is null
+  const int* start_dev;      // [batch]
+  const int* counts;         // [batch] or nullptr
+};
+int launch_kv4_append(const Kv4AppendArgs& args, cudaStream_t stream);
+// Slots [0, n) as bf16 [batch, n, hkv, head_dim].
+int launch_kv4_read(const Kv4Cache& cache, int batch, int n, void* k_out, void* v_out, cudaStream_t stream);
+// One new token of every sequence: its key and value into slot lengths[b], attention over slots [0, lengths[b]], and the
+// weights accumulated where the cache has them.  A length outside [0, max_seq): the output row is zero, nothing else changes.
+struct Kv4AttentionArgs {
+  Kv4Cache cache;
+  const void* qkv;           // [batch, (group + 2) * hkv * head_dim] bf16, row stride in elements
+  long long qkv_stride;
+  void* out;                 // [batch, group * hkv * head_dim] bf16
+  int batch, group;          // group <= 8
+  int length;                // where `lengths` is null
+  const int* lengths;        // [batch]
+  void* workspace;           // kv4_attention_workspace_bytes(...), nothing in it needs to survive the call
+  int num_sms;
+};
+size_t kv4_attention_workspace_bytes(const Kv4Cache& cache, int batch, int group, int num_sms);
+int launch_kv4_attention(const Kv4AttentionArgs& args, cudaStream_t stream);
+// Heads with lengths[b] > keep are cut to `keep` slots; new_lengths[b] = min(lengths[b], keep).
+struct Kv4EvictArgs {
+  Kv4Cache cache;
+  int batch, keep, recent;
+  const int* lengths;        // [batch]
+  int* new_lengths;          // [batch]
+  int* list;                 // [batch * hkv * keep] scratch
+};
+int launch_kv4_evict(const Kv4EvictArgs& args, cudaStream_t stream);
+
 }  // namespace smr

@@ -9,7 +9,7 @@ which at Llama-70B prefill sizes costs more than the o-projection GEMM.
 """
 from __future__ import annotations
 
-from typing import Optional, Union
+from typing import Optional, Sequence, Union
 
 import torch
 
@@ -77,6 +77,21 @@ def rope_(qkv: torch.Tensor, n_heads: int, head_dim: int, seq: int, theta: float
         C.rope_inplace(qkv, int(n_heads), int(head_dim), int(seq), 0, float(theta), _num_sms(qkv.device), pos0)
     else:
         C.rope_inplace(qkv, int(n_heads), int(head_dim), int(seq), int(pos0), float(theta), _num_sms(qkv.device))
+    return qkv
+
+
+@traced("smr.rope_axes_")
+def rope_axes_(qkv: torch.Tensor, n_heads: int, head_dim: int, positions: torch.Tensor, sections: Sequence[int], theta: float,
+               interleaved: bool = False, inverse: bool = False) -> torch.Tensor:
+    """`rope_` with positions of their own: rotate heads `[0, n_heads)` of every row of `qkv` [tokens, row] in place, token t
+    by `positions[:, t]`, one position per axis (int32 [axes, tokens], or [tokens] for one axis; any sign and size).  Pair i
+    of a head, dims `(i, i + head_dim / 2)`, turns by `position * theta ** (-2 i / head_dim)` with the position of one axis:
+    `sections` says how many of the head_dim / 2 pairs each axis has, the first axis the first pairs and so on, or with
+    `interleaved` dealt in turn until an axis has its share.  For images and video the axes are time, row and column; for
+    text all positions of a token are equal, which is plain RoPE.  Angles are exact for every position (64-bit turns), sines
+    fp32, results rounded to bfloat16.  `inverse` rotates back, which is also the gradient of the rotation.  Rows may be
+    strided (on 16 bytes); head_dim is 64 or 128.  Positions are read when the kernel runs."""
+    C.rope_axes(qkv, n_heads, head_dim, positions, sections, theta, interleaved, inverse)
     return qkv
 
 
