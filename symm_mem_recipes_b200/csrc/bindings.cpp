@@ -358,7 +358,7 @@ Kv4Cache kv4_cache(const torch::Tensor& kc, const torch::Tensor& ks, const torch
   for (const torch::Tensor* s : {&ks, &vs})
     need(s->dim() == 4 && s->scalar_type() == torch::kBFloat16 && s->size(0) == kc.size(0) && s->size(1) == kc.size(1) &&
          s->size(2) == slots && s->size(3) == D / 32, "scales must be bfloat16 [batch, kv heads, slots, head_dim / 32]");
-  need(slots % 64 == 0, "a cache has a multiple of 64 slots");
+  need(slots % 64 == 0 && slots <= (1 << 24), "a cache has a multiple of 64 slots, 2^24 at most");
   need(max_seq >= 0 && max_seq <= slots, "max_seq must be at most the cache's ", slots, " slots");
   need(kc.numel() == 0 || kc.size(0) * kc.size(1) * (slots / 64) < (1ll << 30), "the cache has too many tiles");
   need(kc.is_contiguous() && vc.is_contiguous() && ks.is_contiguous() && vs.is_contiguous(), "a cache's tensors must be contiguous");

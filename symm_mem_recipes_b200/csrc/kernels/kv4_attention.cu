@@ -1,6 +1,30 @@
-// One decode step of attention over a 4-bit KV cache (kv4.cuh).
+// One decode step of attention over a 4-bit KV cache (kv4.cuh): append the new token, softmax(q K^T / sqrt(D)) V over
+// sequences of their own lengths, attention weights accumulated.
+//
+// The work is the caches' bytes.  Tiles of 64 slots of all heads and sequences form one list, cut evenly among the grid's
+// warps whatever the lengths are; a warp streams its tiles through a ring in shared memory by asynchronous copies and
+// nothing synchronises warps.  A head whose tiles are all one warp's is finished there, the others leave a piece (maximum,
+// sum, weighted values) per warp, which a second kernel joins in the warps' order: results do not depend on timing.
+//
+// Codes are multiplied as they are.  A nibble in the low bits of a 16-bit float is the subnormal n * 2^-133 (bf16), one in
+// the next four bits sixteen times that, and the tensor cores take subnormals exactly and at full rate (2.4 cycles an
+// MMA and SM, as normal numbers): one AND makes two operands, where a conversion would take three instructions.  Of
+// n = c + 8 the eight is taken out of the sums: in S by an accumulator that starts at -8 sum(q), in the values by one
+// more MMA a group that sums P'.  The cores align addends by their nominal exponents, a subnormal's being 2^-14 (fp16)
+// however small it is: in the lowest bits a nibble would lose ten bits of the sum's 24.  fp16 nibbles therefore stand two bits
+// higher, where the lower one loses six at most, the upper two.
+//
+//   S^T [16 keys x 8 heads] = K q^T, bf16: q is exact, scaled by a power of two per head so that its largest element is
+//   near 2^120; a group's 32 dims are two MMAs, whose sum the key's scale multiplies in fp32.  No operand is rounded.
+//   O^T [16 dims x 8 heads] += V^T P'^T, fp16: P' = 2^(S - M) * scale, where the values' scale of the key and group goes
+//   into the probability.  M is at least (largest S of a tile) + (exponent of its largest scale) - 15, so P' stays below
+//   2^15 and is rounded to 11 bits (2^-12 of itself) down to 2^-29 of the largest; the output is rounded to 8 bits.
+// S^T's accumulators hold heads in rows of four lanes, the second MMA wants keys there: movmatrix transposes in registers.
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include <algorithm>
 
 #include "../device/pdl.cuh"
 #include "kv4.cuh"
@@ -12,20 +36,527 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kThreads = 256;
+constexpr int kWarps = 4;                 // of an attention CTA
+constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
+constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
+constexpr int kJoinThreads = 256;
+constexpr int kJoinTiles = 16;            // tiles whose weights one CTA of the second kernel accumulates
+constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
-__device__ __forceinline__ float key_value(const uint8_t* row, const __nv_bfloat16* scales, int d) {
-  const uint8_t byte = row[(d % 32 / 8) * (D / 8) + (d / 32) * 4 + d % 8 / 2];
-  return __bfloat162float(scales[d / 32]) * (float)((int)(d & 1 ? byte >> 4 : byte & 15) - 8);
-}
-template <int D>
-__device__ __forceinline__ float value_value(const uint8_t* row, const __nv_bfloat16* scales, int d) {
-  const uint8_t byte = row[(d % 32 / 4) * (D / 16) + (d / 32) * 2 + d % 4 / 2];
-  return __bfloat162float(scales[d / 32]) * (float)((int)(d & 1 ? byte >> 4 : byte & 15) - 8);
+struct Layout {
+  static constexpr int kGroups = D / kGroup;
+  static constexpr int kCodes = kTile * D / 2;              // bytes of a tile's codes of keys
+  static constexpr int kScales = kTile * kGroups * 2;       // and of their scales
+  static constexpr int kBytes = 2 * (kCodes + kScales);
+  static constexpr int kStages = kRing / kBytes;
+  static constexpr int kPiece = kHeads * (D + 2);           // floats: maxima, sums, weighted values [head][D]
+};
+
+// The calls' scratch: pieces of the warps, (M, l) of the heads that one warp finished, scores of all tiles.
+struct Workspace {
+  float* pieces;      // [warps][2][kPiece]: a warp's first head and its last one, where they are shared with others
+  float2* stats;      // [batch * hkv][kHeads]
+  float* scores;      // [tiles][kTile][padded group], units of log2
+};
+__host__ __device__ inline int padded_group(int group) { return (group + 1) & ~1; }
+__host__ __device__ inline Workspace carve(void* base, int head_dim, int batch_heads, int warps) {
+  Workspace w;
+  w.pieces = static_cast<float*>(base);
+  w.stats = reinterpret_cast<float2*>(w.pieces + (size_t)warps * 2 * kHeads * (head_dim + 2));
+  w.scores = reinterpret_cast<float*>(w.stats + (size_t)batch_heads * kHeads);
+  return w;
 }
 
-__device__ float block_reduce(float v, bool is_max, float* buf) {
+__device__ __forceinline__ int length_of(const Kv4AttentionArgs& a, int b) { return a.lengths ? a.lengths[b] : a.length; }
+// Tiles of a head of sequence b, the new token's included; none for an idle sequence.
+__device__ __forceinline__ int tiles_of(const Kv4AttentionArgs& a, int b) {
+  const int n = length_of(a, b);
+  return n >= 0 && n < a.cache.max_seq ? n / kTile + 1 : 0;
+}
+// First tile of a warp, and the warp that has a tile.
+__device__ __forceinline__ int first_tile(long long tiles, int warps, int w) { return (int)(tiles * w / warps); }
+__device__ __forceinline__ int warp_of(long long tiles, int warps, int tile) {
+  return (int)(((long long)(tile + 1) * warps - 1) / tiles);
+}
+
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_fp16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_of(float lo, float hi) {
+  uint32_t y;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(y) : "f"(hi), "f"(lo));
+  return y;
+}
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float lo_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 << 16); }
+__device__ __forceinline__ float hi_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 & 0xFFFF0000u); }
+
+// Where a warp is in the list of tiles.
+struct Cursor {
+  int b, h, t, n;      // sequence, kv head, tile of it, tiles of the head
+};
+
+// Row of a tile that stands in row `rho` of the MMAs' 16 keys: neighbours keep opposite parity, and so do rows 0, 2, 4, 6, for
+// shared memory's banks (64 bytes a row at D = 128).
+__device__ __forceinline__ int row_of(int rho) { return rho ^ ((rho >> 1) & 1); }
+
+template <int D, bool kScores>
+struct Attend {
+  using L = Layout<D>;
+  static constexpr int kG = L::kGroups;
+
+  // Lane (r = lane / 4, c = lane % 4).  q: operand B, head r, dims 32 g + 8 c + .. in the codes' order: of a word's nibbles
+  // j and j + 4 make a pair; [g][half][b0 / b1].
+  uint32_t q[kG][2][2];
+  float minus8[kG][2];      // accumulators' start for heads 2c, 2c + 1
+  float to_log2[2];         // S in the accumulators' units -> units of log2
+  float m[2], l[2];         // M, and this lane's rows' share of the sum, of heads 2c and 2c + 1
+  float acc[kG][2][4];      // [g][t]: dims 32 g + 4 r + 2 t (first two, 2^-22 n P') and the next one (last two, 2^-18 n P')
+  float sum[kG][4];         // sum of P'
+
+  __device__ __forceinline__ void start(const Kv4AttentionArgs& a, int b, int h) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.qkv) + (size_t)b * a.qkv_stride +
+                               ((size_t)h * a.group + r) * D + 8 * c;
+    Vec16 raw[kG];
+#pragma unroll
+    for (int g = 0; g < kG; ++g) raw[g] = r < a.group ? ld_16_nc(row + kGroup * g) : Vec16{0, 0, 0, 0};
+    float largest = 0.0f;
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i == 0 ? raw[g].x : i == 1 ? raw[g].y : i == 2 ? raw[g].z : raw[g].w;
+        largest = fmaxf(largest, fmaxf(fabsf(lo_of(w)), fabsf(hi_of(w))));
+      }
+    }
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+    // 2^(120 - e): the largest element comes to [2^120, 2^121); e is held in [-6, 127], where the factor is a normal number
+    const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -6), 127);
+    const float up = __uint_as_float((uint32_t)(120 - e + 127) << 23);
+    // S = 2^-133 n 2^(120 - e) q: back by 2^(13 + e), then log2(e) / sqrt(D)
+    const float back = ldexpf(kLog2e * rsqrtf((float)D), 13 + e);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) to_log2[j] = __shfl_sync(0xffffffffu, back, 4 * (2 * c + j));
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+      const uint32_t w[4] = {raw[g].x, raw[g].y, raw[g].z, raw[g].w};
+      float f[8], sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        f[2 * i] = lo_of(w[i]) * up;
+        f[2 * i + 1] = hi_of(w[i]) * up;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += f[i];
+      // nibbles 0, 4 | 1, 5 (times 16) of the word, then 2, 6 | 3, 7; a multiplication by a power of two rounds nothing
+      q[g][0][0] = pack_bf16x2(f[0], f[4]);
+      q[g][0][1] = pack_bf16x2(f[1] * 0.0625f, f[5] * 0.0625f);
+      q[g][1][0] = pack_bf16x2(f[2], f[6]);
+      q[g][1][1] = pack_bf16x2(f[3] * 0.0625f, f[7] * 0.0625f);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+      sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      sum *= -0.0625f;                               // -8 * 2^-133 as -2^-4 and 2^-126
+      sum *= 1.1754943508222875e-38f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) minus8[g][j] = __shfl_sync(0xffffffffu, sum, 4 * (2 * c + j));
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      m[j] = -INFINITY;
+      l[j] = 0.0f;
+    }
+#pragma unroll
+    for (int g = 0; g < kG; ++g) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[g][0][i] = acc[g][1][i] = sum[g][i] = 0.0f;
+    }
+  }
+
+  // One tile in shared memory; the first `valid` slots are seen.  `scores`: where the tile's scores go.
+  __device__ __forceinline__ void tile(const uint8_t* stage, int valid, float* scores, int group, int pitch) {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const uint8_t* kc = stage;
+    const uint8_t* vc = stage + L::kCodes;
+    const uint8_t* ks = stage + 2 * L::kCodes;
+    const uint8_t* vs = ks + L::kScales;
+    float s[4][4];
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+      uint32_t w[2][kG], sc[2][kG / 2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = sub * 16 + row_of(r) + 8 * j;
+        const uint8_t* p = kc + row * (D / 2) + c * (D / 8);
+        const uint8_t* ps = ks + row * (2 * kG);
+        if constexpr (D == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p);
+          w[j][0] = x.x; w[j][1] = x.y; w[j][2] = x.z; w[j][3] = x.w;
+          const uint2 y = *reinterpret_cast<const uint2*>(ps);
+          sc[j][0] = y.x; sc[j][1] = y.y;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(p);
+          w[j][0] = x.x; w[j][1] = x.y;
+          sc[j][0] = *reinterpret_cast<const uint32_t*>(ps);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        float d[4] = {minus8[g][0], minus8[g][1], minus8[g][0], minus8[g][1]};
+        const uint32_t x = w[0][g], y = w[1][g];
+        mma_bf16(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[g][0][0], q[g][0][1]);
+        mma_bf16(d, x >> 8 & 0x000F000Fu, y >> 8 & 0x000F000Fu, x >> 8 & 0x00F000F0u, y >> 8 & 0x00F000F0u, q[g][1][0],
+                 q[g][1][1]);
+        const float sx = g & 1 ? hi_of(sc[0][g / 2]) : lo_of(sc[0][g / 2]);
+        const float sy = g & 1 ? hi_of(sc[1][g / 2]) : lo_of(sc[1][g / 2]);
+        s[sub][0] = g == 0 ? d[0] * sx : fmaf(d[0], sx, s[sub][0]);
+        s[sub][1] = g == 0 ? d[1] * sx : fmaf(d[1], sx, s[sub][1]);
+        s[sub][2] = g == 0 ? d[2] * sy : fmaf(d[2], sy, s[sub][2]);
+        s[sub][3] = g == 0 ? d[3] * sy : fmaf(d[3], sy, s[sub][3]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[sub][i] *= to_log2[i & 1];
+      if constexpr (kScores) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = sub * 16 + row_of(r) + 8 * j;
+          if (2 * c < group && row < valid)
+            *reinterpret_cast<float2*>(scores + row * pitch + 2 * c) = make_float2(s[sub][2 * j], s[sub][2 * j + 1]);
+        }
+      }
+    }
+    // scales of the values of this lane's rows; a row that is not seen has a score of minus infinity and scales of zero
+    uint32_t sv[4][2][kG / 2];
+    __nv_bfloat162 top2 = __float2bfloat162_rn(0.0f);
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int row = sub * 16 + row_of(r) + 8 * j;
+        const uint8_t* ps = vs + row * (2 * kG);
+        if constexpr (D == 128) {
+          const uint2 y = *reinterpret_cast<const uint2*>(ps);
+          sv[sub][j][0] = y.x; sv[sub][j][1] = y.y;
+        } else {
+          sv[sub][j][0] = *reinterpret_cast<const uint32_t*>(ps);
+        }
+        if (valid < kTile && row >= valid) {
+#pragma unroll
+          for (int i = 0; i < kG / 2; ++i) sv[sub][j][i] = 0;
+          s[sub][2 * j] = s[sub][2 * j + 1] = -INFINITY;
+        }
+#pragma unroll
+        for (int i = 0; i < kG / 2; ++i)      // of a NaN and a number this is the number
+          top2 = __hmax2(top2, *reinterpret_cast<const __nv_bfloat162*>(&sv[sub][j][i]));
+      }
+    }
+    float top = fmaxf(__low2float(top2), __high2float(top2));
+    float high[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      high[j] = fmaxf(fmaxf(fmaxf(s[0][j], s[0][j + 2]), fmaxf(s[1][j], s[1][j + 2])),
+                      fmaxf(fmaxf(s[2][j], s[2][j + 2]), fmaxf(s[3][j], s[3][j + 2])));
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      high[0] = fmaxf(high[0], __shfl_xor_sync(0xffffffffu, high[0], o));
+      high[1] = fmaxf(high[1], __shfl_xor_sync(0xffffffffu, high[1], o));
+    }
+    // 2^(e - 126) is above the largest scale; below 2^-60 it does not matter
+    const float exponent = (float)(max((int)(__float_as_uint(top) >> 23), 66) - 126 - 15);
+    const float m0 = fmaxf(m[0], high[0] + exponent), m1 = fmaxf(m[1], high[1] + exponent);
+    if (__any_sync(0xffffffffu, m0 != m[0] || m1 != m[1])) {
+      const float f0 = exp2_of(m[0] - m0), f1 = exp2_of(m[1] - m1);
+      m[0] = m0;
+      m[1] = m1;
+      l[0] *= f0;
+      l[1] *= f1;
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[g][0][i] *= i & 1 ? f1 : f0;
+          acc[g][1][i] *= i & 1 ? f1 : f0;
+          sum[g][i] *= i & 1 ? f1 : f0;
+        }
+      }
+    }
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[sub][i] = exp2_of(s[sub][i] - m[i & 1]);
+        l[i & 1] += s[sub][i];
+      }
+    }
+#pragma unroll
+    for (int sub = 0; sub < 4; ++sub) {
+      uint32_t x[4][kG / 2];      // this lane's part of the values of MMA rows 2c, 2c + 1, 2c + 8, 2c + 9
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint8_t* p = vc + (sub * 16 + row_of(2 * c + (k & 1)) + 8 * (k >> 1)) * (D / 2) + r * (D / 16);
+        if constexpr (D == 128) {
+          const uint2 y = *reinterpret_cast<const uint2*>(p);
+          x[k][0] = y.x; x[k][1] = y.y;
+        } else {
+          x[k][0] = *reinterpret_cast<const uint32_t*>(p);
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g) {
+        const float sx = g & 1 ? hi_of(sv[sub][0][g / 2]) : lo_of(sv[sub][0][g / 2]);
+        const float sy = g & 1 ? hi_of(sv[sub][1][g / 2]) : lo_of(sv[sub][1][g / 2]);
+        const uint32_t b0 = transpose_8x8(half2_of(s[sub][0] * sx, s[sub][1] * sx));
+        const uint32_t b1 = transpose_8x8(half2_of(s[sub][2] * sy, s[sub][3] * sy));
+        const uint32_t y0 = __byte_perm(x[0][g / 2], x[1][g / 2], g & 1 ? 0x7632 : 0x5410);
+        const uint32_t y1 = __byte_perm(x[2][g / 2], x[3][g / 2], g & 1 ? 0x7632 : 0x5410);
+        mma_fp16(acc[g][0], y0 << 2 & 0x003C003Cu, y0 << 2 & 0x03C003C0u, y1 << 2 & 0x003C003Cu, y1 << 2 & 0x03C003C0u, b0, b1);
+        mma_fp16(acc[g][1], y0 >> 6 & 0x003C003Cu, y0 >> 6 & 0x03C003C0u, y1 >> 6 & 0x003C003Cu, y1 >> 6 & 0x03C003C0u, b0, b1);
+        mma_fp16(sum[g], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0, b1);
+      }
+    }
+  }
+
+  // Weighted values of head 2c + j: dims 32 g + 4 r .. + 3.
+  __device__ __forceinline__ float4 values(int g, int j) const {
+    constexpr float kEven = 4194304.0f, kOdd = 262144.0f;      // 2^22, 2^18
+    const float e = 8.0f * sum[g][j];
+    return make_float4(fmaf(acc[g][0][j], kEven, -e), fmaf(acc[g][0][2 + j], kOdd, -e), fmaf(acc[g][1][j], kEven, -e),
+                       fmaf(acc[g][1][2 + j], kOdd, -e));
+  }
+  __device__ __forceinline__ void join_lanes() {
+#pragma unroll
+    for (int o = 4; o <= 16; o <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], o);
+    }
+  }
+};
+
+// The new token's row, four dims a lane: into the tile in shared memory and into the cache.
+template <int D>
+__device__ __forceinline__ void append_row(const Kv4AttentionArgs& a, int b, int h, int slot, uint8_t* stage) {
+  using L = Layout<D>;
+  const int lane = threadIdx.x & 31, g = lane >> 3, hkv = a.cache.hkv;
+  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.qkv) + (size_t)b * a.qkv_stride + (size_t)a.group * hkv * D;
+  const size_t at = ((size_t)b * hkv + h) * a.cache.slots + slot;
+  const int in_tile = slot % kTile;
+#pragma unroll
+  for (int kind = 0; kind < 2; ++kind) {
+    uint2 raw = make_uint2(0, 0);
+    if (lane < D / 4) raw = *reinterpret_cast<const uint2*>(row + ((size_t)kind * hkv + h) * D + 4 * lane);
+    const float f[4] = {lo_of(raw.x), hi_of(raw.x), lo_of(raw.y), hi_of(raw.y)};
+    float largest = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      finite = finite && is_finite(f[i]);
+      largest = fmaxf(largest, fabsf(f[i]));
+    }
+    if (!finite) largest = INFINITY;
+#pragma unroll
+    for (int o = 1; o <= 4; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const Scale s = scale_of(largest, is_finite(largest));
+    uint32_t half = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) half |= nibble_of(f[i], s) << (4 * i);
+    if (lane < D / 4) {
+      const int byte = kind == 0 ? (lane & 7) / 2 * (D / 8) + g * 4 + (lane & 1) * 2 : (lane & 7) * (D / 16) + g * 2;
+      uint8_t* codes = kind == 0 ? a.cache.k_codes : a.cache.v_codes;
+      *reinterpret_cast<uint16_t*>(codes + at * (D / 2) + byte) = (uint16_t)half;
+      *reinterpret_cast<uint16_t*>(stage + kind * L::kCodes + in_tile * (D / 2) + byte) = (uint16_t)half;
+      if ((lane & 7) == 0) {
+        static_cast<__nv_bfloat16*>(kind == 0 ? a.cache.k_scales : a.cache.v_scales)[at * L::kGroups + g] = s.s;
+        reinterpret_cast<__nv_bfloat16*>(stage + 2 * L::kCodes + kind * L::kScales)[in_tile * L::kGroups + g] = s.s;
+      }
+    }
+  }
+}
+
+template <int D, bool kScores>
+__global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_constant__ Kv4AttentionArgs a) {
+  using L = Layout<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int warp_sums[kWarps];
+  int* start = reinterpret_cast<int*>(smem + kWarps * kRing);      // [batch + 1]: first tile of a sequence
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hkv = a.cache.hkv;
+  pdl_wait();
+  pdl_launch_dependents();
+  {
+    const int per = (a.batch + 32 * kWarps - 1) / (32 * kWarps), b0 = threadIdx.x * per;
+    int sum = 0;
+    for (int i = 0; i < per; ++i) sum += b0 + i < a.batch ? tiles_of(a, b0 + i) * hkv : 0;
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sums[warp] = x;
+    __syncthreads();
+    int before = x - sum;
+    for (int i = 0; i < warp; ++i) before += warp_sums[i];
+    for (int i = 0; i < per && b0 + i < a.batch; ++i) {
+      start[b0 + i] = before;
+      before += tiles_of(a, b0 + i) * hkv;
+    }
+    if (threadIdx.x == 32 * kWarps - 1) start[a.batch] = before;
+    __syncthreads();
+  }
+  const long long tiles = start[a.batch];
+  if (tiles == 0) return;
+  const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
+  const int first = first_tile(tiles, warps, w), end = first_tile(tiles, warps, w + 1);
+  if (first == end) return;
+  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
+
+  Cursor now;
+  {
+    int lo = 0, hi = a.batch;      // the last sequence that starts at `first` or before and has tiles
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (start[mid] <= first) lo = mid;
+      else hi = mid;
+    }
+    now.b = lo;
+    now.n = (start[lo + 1] - start[lo]) / hkv;
+    now.h = (first - start[lo]) / now.n;
+    now.t = first - start[lo] - now.h * now.n;
+  }
+  auto advance = [&](Cursor& at) {
+    if (++at.t < at.n) return;
+    at.t = 0;
+    if (++at.h < hkv) return;
+    at.h = 0;
+    do {
+      ++at.b;
+    } while (at.b < a.batch && start[at.b + 1] == start[at.b]);
+    if (at.b < a.batch) at.n = (start[at.b + 1] - start[at.b]) / hkv;
+  };
+  uint8_t* ring = smem + warp * kRing;
+  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+  auto fetch = [&](const Cursor& at, int stage) {
+    const size_t slot = ((size_t)at.b * hkv + at.h) * a.cache.slots + (size_t)at.t * kTile;
+    const uint32_t dst = ring_addr + stage * L::kBytes + lane * 16;
+    const uint8_t* kc = a.cache.k_codes + slot * (D / 2) + lane * 16;
+    const uint8_t* vc = a.cache.v_codes + slot * (D / 2) + lane * 16;
+#pragma unroll
+    for (int i = 0; i < L::kCodes / 512; ++i) {
+      copy_async_16(dst + i * 512, kc + i * 512);
+      copy_async_16(dst + L::kCodes + i * 512, vc + i * 512);
+    }
+    const uint8_t* ks = static_cast<const uint8_t*>(a.cache.k_scales) + slot * (2 * L::kGroups);
+    const uint8_t* vs = static_cast<const uint8_t*>(a.cache.v_scales) + slot * (2 * L::kGroups);
+    if constexpr (D == 128) {
+      copy_async_16(dst + 2 * L::kCodes, ks + lane * 16);
+      copy_async_16(dst + 2 * L::kCodes + L::kScales, vs + lane * 16);
+    } else {      // 256 bytes of either, half a warp each
+      copy_async_16(dst + 2 * L::kCodes, lane < 16 ? ks + lane * 16 : vs + (lane - 16) * 16);
+    }
+  };
+  Cursor ahead = now;
+  int to_fetch = first;
+#pragma unroll
+  for (int i = 0; i < L::kStages - 1; ++i) {
+    if (to_fetch < end) {
+      fetch(ahead, i);
+      advance(ahead);
+      ++to_fetch;
+    }
+    copy_commit();
+  }
+
+  Attend<D, kScores> at;
+  const int pitch = padded_group(a.group);
+  bool first_head = true, whole = now.t == 0;      // `whole`: this warp has the head's tiles from the first on
+  int stage = 0;
+  for (int i = first; i < end; ++i) {
+    if (now.t == 0 || i == first) at.start(a, now.b, now.h);
+    copy_wait<L::kStages - 2>();
+    __syncwarp();      // the tile is there for every lane, and every lane is done with the stage that is filled next
+    if (to_fetch < end) {
+      fetch(ahead, stage == 0 ? L::kStages - 1 : stage - 1);
+      advance(ahead);
+      ++to_fetch;
+    }
+    copy_commit();
+    uint8_t* buf = ring + stage * L::kBytes;
+    const bool last = now.t == now.n - 1;
+    int valid = kTile;
+    if (last) {
+      const int slot = length_of(a, now.b);
+      valid = slot % kTile + 1;
+      append_row<D>(a, now.b, now.h, slot, buf);
+      __syncwarp();
+    }
+    at.tile(buf, valid, ws.scores + (size_t)i * kTile * pitch, a.group, pitch);
+    stage = stage == L::kStages - 1 ? 0 : stage + 1;
+    if (last || i + 1 == end) {
+      at.join_lanes();
+      const int r = lane >> 2, c = lane & 3;
+      const bool finished = last && whole;
+      float* piece = ws.pieces + ((size_t)w * 2 + (first_head ? 0 : 1)) * L::kPiece;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int head = 2 * c + j;
+        if (head >= a.group) continue;
+        if (finished) {
+          const float inv = 1.0f / at.l[j];
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (((size_t)now.b * hkv + now.h) * a.group + head) * D + 4 * r;
+#pragma unroll
+          for (int g = 0; g < L::kGroups; ++g) {
+            const float4 v = at.values(g, j);
+            *reinterpret_cast<uint2*>(out + kGroup * g) =
+                make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
+          }
+          if (kScores && r == 0)
+            ws.stats[((size_t)now.b * hkv + now.h) * kHeads + head] = make_float2(at.m[j], at.l[j]);
+        } else {
+          if (r == 0) {
+            piece[head] = at.m[j];
+            piece[kHeads + head] = at.l[j];
+          }
+#pragma unroll
+          for (int g = 0; g < L::kGroups; ++g)
+            *reinterpret_cast<float4*>(piece + 2 * kHeads + head * D + kGroup * g + 4 * r) = at.values(g, j);
+        }
+      }
+      first_head = false;
+      whole = true;
+    }
+    advance(now);
+  }
+}
+
+__device__ __forceinline__ float block_reduce(float v, bool is_max, float* buf) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -36,107 +567,198 @@ __device__ float block_reduce(float v, bool is_max, float* buf) {
   if (lane == 0) buf[warp] = v;
   __syncthreads();
   float r = buf[0];
-  for (int i = 1; i < kThreads / 32; ++i) r = is_max ? fmaxf(r, buf[i]) : r + buf[i];
+#pragma unroll
+  for (int i = 1; i < kJoinThreads / 32; ++i) r = is_max ? fmaxf(r, buf[i]) : r + buf[i];
   return r;
 }
 
-// One CTA a (sequence, kv head): append, scores into the workspace, softmax, weights, output.
-template <int D>
-__global__ void __launch_bounds__(kThreads) attend_kernel(Kv4AttentionArgs a) {
+// blockIdx.x: (sequence, kv head).  blockIdx.y < group: joins the pieces of that query head, where the head was cut.
+// blockIdx.y >= group: accumulates the weights of kJoinTiles tiles.
+template <int D, bool kScores>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Kv4AttentionArgs a, int warps) {
+  using L = Layout<D>;
+  __shared__ float buf[kJoinThreads / 32];
+  __shared__ int sums[2][kJoinThreads / 32];
+  __shared__ float norms[2][kHeads], part[kJoinThreads / 32][kHeads];
+  __shared__ float4 halves[kJoinThreads / (D / 4)][D / 4];
+  const int bh = blockIdx.x, hkv = a.cache.hkv, b = bh / hkv, h = bh % hkv, tid = threadIdx.x;
   pdl_wait();
-  __shared__ float q[8][D];
-  __shared__ float buf[kThreads / 32];
-  __shared__ float norm[8];
-  const int head = blockIdx.x, hkv = a.cache.hkv, b = head / hkv, h = head % hkv, g = a.group, tid = threadIdx.x;
-  const int len = a.lengths ? a.lengths[b] : a.length;
-  const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(a.qkv) + (size_t)b * a.qkv_stride;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((size_t)b * hkv + h) * g * D;
-  if (len < 0 || len >= a.cache.max_seq) {
-    for (int i = tid; i < g * D; i += kThreads) out[i] = __float2bfloat16_rn(0.0f);
+  const int n = tiles_of(a, b);
+  if (n == 0) {      // idle: the output row is zero
+    if ((int)blockIdx.y < a.group && tid < D / 8)
+      st_16(static_cast<__nv_bfloat16*>(a.out) + ((size_t)bh * a.group + blockIdx.y) * D + tid * 8, Vec16{0, 0, 0, 0});
     return;
   }
-  for (int i = tid; i < g * D; i += kThreads) q[i / D][i % D] = __bfloat162float(row[h * g * D + i]);
-  const size_t base = (size_t)head * a.cache.slots;
-  __nv_bfloat16* ks = static_cast<__nv_bfloat16*>(a.cache.k_scales) + base * (D / kGroup);
-  __nv_bfloat16* vs = static_cast<__nv_bfloat16*>(a.cache.v_scales) + base * (D / kGroup);
-  uint8_t* kc = a.cache.k_codes + base * (D / 2);
-  uint8_t* vc = a.cache.v_codes + base * (D / 2);
-  if (tid < 2 * (D / kGroup)) {
-    const bool is_value = tid >= D / kGroup;
-    const int grp = tid % (D / kGroup);
-    const __nv_bfloat16* src = row + (a.group * hkv + (is_value ? hkv : 0) + h) * D + grp * kGroup;
-    float largest = 0.0f;
-    bool finite = true;
-    for (int i = 0; i < kGroup; ++i) {
-      const float x = __bfloat162float(src[i]);
-      finite = finite && is_finite(x);
-      largest = fmaxf(largest, fabsf(x));
-    }
-    const Scale s = scale_of(largest, finite);
-    (is_value ? vs : ks)[(size_t)len * (D / kGroup) + grp] = s.s;
-    for (int i = 0; i < kGroup; i += 2) {
-      const uint32_t byte = nibble_of(__bfloat162float(src[i]), s) | nibble_of(__bfloat162float(src[i + 1]), s) << 4;
-      if (is_value) vc[(size_t)len * (D / 2) + (i / 4) * (D / 16) + grp * 2 + i % 4 / 2] = (uint8_t)byte;
-      else kc[(size_t)len * (D / 2) + (i / 8) * (D / 8) + grp * 4 + i % 8 / 2] = (uint8_t)byte;
-    }
+  const int chunk = (int)blockIdx.y - a.group;
+  if (kScores && chunk >= 0 && chunk * kJoinTiles >= n) return;
+  int before = 0, all = 0;
+  for (int i = tid; i < a.batch; i += kJoinThreads) {
+    const int t = tiles_of(a, i);
+    all += t;
+    before += i < b ? t : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+  }
+  if ((tid & 31) == 0) {
+    sums[0][tid >> 5] = before;
+    sums[1][tid >> 5] = all;
   }
   __syncthreads();
-  const int n = len + 1;
-  float* score = static_cast<float*>(a.workspace) + base * g;
-  float top[8];
-  for (int j = 0; j < g; ++j) top[j] = -INFINITY;
-  for (int i = tid; i < n; i += kThreads) {
-    float s[8] = {};
-    for (int d = 0; d < D; ++d) {
-      const float k = key_value<D>(kc + (size_t)i * (D / 2), ks + (size_t)i * (D / kGroup), d);
-      for (int j = 0; j < g; ++j) s[j] += q[j][d] * k;
-    }
-    for (int j = 0; j < g; ++j) {
-      s[j] *= rsqrtf((float)D);
-      score[(size_t)i * g + j] = s[j];
-      top[j] = fmaxf(top[j], s[j]);
-    }
+  before = all = 0;
+#pragma unroll
+  for (int i = 0; i < kJoinThreads / 32; ++i) {
+    before += sums[0][i];
+    all += sums[1][i];
   }
-  for (int j = 0; j < g; ++j) {
-    const float m = block_reduce(top[j], true, buf);
+  const long long tiles = (long long)all * hkv;
+  const int s0 = before * hkv + h * n, s1 = s0 + n;
+  const int wa = warp_of(tiles, warps, s0), wb = warp_of(tiles, warps, s1 - 1);
+  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
+  // the piece of warp w, or null if it has no tiles
+  auto piece_of = [&](int w) -> const float* {
+    const int f = first_tile(tiles, warps, w);
+    if (f == first_tile(tiles, warps, w + 1)) return nullptr;
+    return ws.pieces + ((size_t)w * 2 + (f < s0 ? 1 : 0)) * L::kPiece;
+  };
+  if (chunk < 0) {
+    if (wa == wb) return;
+    const int q = blockIdx.y;
+    float m = -INFINITY;
+    for (int w = wa + tid; w <= wb; w += kJoinThreads) {
+      const float* p = piece_of(w);
+      if (p != nullptr) m = fmaxf(m, p[q]);
+    }
+    m = block_reduce(m, true, buf);
+    // D / 4 threads a piece, four dims each
+    constexpr int kSide = kJoinThreads / (D / 4);
+    const int side = tid / (D / 4), d = tid % (D / 4);
+    float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     float sum = 0.0f;
-    for (int i = tid; i < n; i += kThreads) {
-      const float p = __expf(score[(size_t)i * g + j] - m);
-      score[(size_t)i * g + j] = p;
-      sum += p;
+#pragma unroll 4
+    for (int w = wa + side; w <= wb; w += kSide) {
+      const float* p = piece_of(w);
+      if (p == nullptr) continue;
+      const float f = exp2_of(p[q] - m);
+      const float4 v = *reinterpret_cast<const float4*>(p + 2 * kHeads + q * D + 4 * d);
+      o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+      if (d == 0) sum += f * p[kHeads + q];
     }
-    sum = block_reduce(sum, false, buf);
-    if (tid == 0) norm[j] = 1.0f / sum;
+    halves[side][d] = o;
+    sum = block_reduce(sum, false, buf);      // synchronises
+    if (side == 0) {
+      for (int i = 1; i < kSide; ++i) {
+        o.x += halves[i][d].x; o.y += halves[i][d].y; o.z += halves[i][d].z; o.w += halves[i][d].w;
+      }
+      const float inv = 1.0f / sum;
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + ((size_t)bh * a.group + q) * D + 4 * d) =
+          make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+    }
+    return;
   }
-  __syncthreads();
-  if (a.cache.weights != nullptr) {
-    float* w = a.cache.weights + base;
-    for (int i = tid; i < n; i += kThreads) {
-      float sum = 0.0f;
-      for (int j = 0; j < g; ++j) sum += score[(size_t)i * g + j] * norm[j];
-      w[i] = i == len ? sum : w[i] + sum;
+  if constexpr (kScores) {
+    const int q = tid % kHeads;
+    if (wa == wb) {
+      if (tid < kHeads && q < a.group) {
+        const float2 s = ws.stats[(size_t)bh * kHeads + q];
+        norms[0][q] = s.x;
+        norms[1][q] = 1.0f / s.y;
+      }
+    } else {
+      float m = -INFINITY, sum = 0.0f;
+      if (q < a.group)
+        for (int w = wa + tid / kHeads; w <= wb; w += kJoinThreads / kHeads) {
+          const float* p = piece_of(w);
+          if (p != nullptr) m = fmaxf(m, p[q]);
+        }
+#pragma unroll
+      for (int o = kHeads; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      if ((tid & 31) < kHeads) part[tid >> 5][q] = m;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, part[i][q]);
+      __syncthreads();
+      if (q < a.group)
+        for (int w = wa + tid / kHeads; w <= wb; w += kJoinThreads / kHeads) {
+          const float* p = piece_of(w);
+          if (p != nullptr) sum += exp2_of(p[q] - m) * p[kHeads + q];
+        }
+#pragma unroll
+      for (int o = kHeads; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if ((tid & 31) < kHeads) part[tid >> 5][q] = sum;
+      __syncthreads();
+      if (tid < kHeads) {
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kJoinThreads / 32; ++i) sum += part[i][q];
+        norms[0][q] = m;
+        norms[1][q] = 1.0f / sum;
+      }
+    }
+    __syncthreads();
+    const int pitch = padded_group(a.group), len = length_of(a, b);
+    const int end = min(len + 1, (chunk + 1) * kJoinTiles * kTile);
+    float* weights = a.cache.weights + (size_t)bh * a.cache.slots;
+    const float* scores = ws.scores + (size_t)s0 * kTile * pitch;
+    for (int i = chunk * kJoinTiles * kTile + tid; i < end; i += kJoinThreads) {
+      const float2* s = reinterpret_cast<const float2*>(scores + (size_t)i * pitch);
+      float p = 0.0f;
+      for (int j = 0; j < a.group; j += 2) {
+        const float2 x = s[j / 2];
+        p += exp2_of(x.x - norms[0][j]) * norms[1][j];
+        if (j + 1 < a.group) p += exp2_of(x.y - norms[0][j + 1]) * norms[1][j + 1];
+      }
+      weights[i] = i == len ? p : weights[i] + p;
     }
   }
-  for (int e = tid; e < g * D; e += kThreads) {
-    const int j = e / D, d = e % D;
-    float o = 0.0f;
-    for (int i = 0; i < n; ++i)
-      o += score[(size_t)i * g + j] * value_value<D>(vc + (size_t)i * (D / 2), vs + (size_t)i * (D / kGroup), d);
-    out[e] = __float2bfloat16_rn(o * norm[j]);
-  }
+}
+
+int attention_ctas(const Kv4Cache& cache, int batch, int num_sms) {
+  const long long tiles = (long long)batch * cache.hkv * (cache.slots / kTile);
+  return (int)std::max<long long>(1, std::min<long long>(2ll * num_sms, (tiles + kWarps - 1) / kWarps));
+}
+
+template <int D, bool kScores>
+int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
+  const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
+  const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
+  int e = (int)cudaFuncSetAttribute(attend_kernel<D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e != 0) return e;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(32 * kWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  e = (int)cudaLaunchKernelEx(&cfg, attend_kernel<D, kScores>, a);
+  if (e != 0) return e;
+  const int chunks = kScores ? (a.cache.slots / kTile + kJoinTiles - 1) / kJoinTiles : 0;
+  cfg.gridDim = dim3(a.batch * a.cache.hkv, a.group + chunks);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  return (int)cudaLaunchKernelEx(&cfg, join_kernel<D, kScores>, a, ctas * kWarps);
 }
 
 }  // namespace
 
-size_t kv4_attention_workspace_bytes(const Kv4Cache& cache, int batch, int group, int) {
-  return (size_t)batch * cache.hkv * cache.slots * group * sizeof(float);
+size_t kv4_attention_workspace_bytes(const Kv4Cache& cache, int batch, int group, int num_sms) {
+  const size_t warps = (size_t)attention_ctas(cache, batch, num_sms) * kWarps;
+  size_t bytes = warps * 2 * kHeads * (cache.head_dim + 2) * sizeof(float) + (size_t)batch * cache.hkv * kHeads * sizeof(float2);
+  if (cache.weights != nullptr) bytes += (size_t)batch * cache.hkv * cache.slots * padded_group(group) * sizeof(float);
+  return bytes;
 }
 
 int launch_kv4_attention(const Kv4AttentionArgs& a, cudaStream_t stream) {
   if (a.batch == 0) return 0;
-  if (a.cache.head_dim == 128) attend_kernel<128><<<a.batch * a.cache.hkv, kThreads, 0, stream>>>(a);
-  else attend_kernel<64><<<a.batch * a.cache.hkv, kThreads, 0, stream>>>(a);
-  return (int)cudaGetLastError();
+  const bool scores = a.cache.weights != nullptr;
+  if (a.cache.head_dim == 128) return scores ? launch<128, true>(a, stream) : launch<128, false>(a, stream);
+  return scores ? launch<64, true>(a, stream) : launch<64, false>(a, stream);
 }
 
 }  // namespace smr

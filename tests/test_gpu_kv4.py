@@ -5,7 +5,15 @@ sine and cosine are off by 2^-21.1 (the intrinsic's bound on [-pi, pi]) and 2^-2
 and three fp32 roundings add 3 * 2^-24: 2^-19.5 (|x| + |y|) covers both.  A score is a sum of head_dim <= 128 fp32 products in
 at most 64 dependent steps: off by 2^-18 A, A the largest sum |q k| / sqrt(D), and so is p relative to itself, twice
 (numerator and sum), with 2^-20 for the exponential; the probabilities may be rounded to fp16 (2^-11) on their way into the
-weighted sum, which adds 2^-18 of sum p |v| for its own steps."""
+weighted sum, which adds 2^-18 of sum p |v| for its own steps.
+
+Both sums may be taken over nibbles n = c + 8 in [1, 15] by tensor cores, with 8 sum(q s) or 8 sum(p s) taken off.  An MMA adds 17
+numbers, each cut at 2^-24 of twice the largest nominal product or of the accumulator.  Products: a nibble may be a subnormal of
+bf16 (nominal 2^-126, unit 2^-133) or one of fp16 (2^-14, unit 2^-22): 17 * 2^-24 * 2^8 = 2^-11.9 of the largest |q| s, two MMAs a
+group of 32 dims, so 2^-10.9 max|q| sum_g s / sqrt(D) in a score; 17 * 2^-24 * 2^9 = 2^-10.9 of p s, and the largest p s
+of each MMA add up to no more than sum p s.  Accumulators: k of them in a chain lose k * 2^-23 of the total, 15 sum p s, and of 8
+sum p s: k * 2^-18.4 sum p s.  A warp has four such MMAs a tile of 64 slots and goes on to a second tile once the work has more
+tiles than warps: k = 8 for up to 512 tiles in all and 8 more for every further 512 is no less."""
 import math
 
 import pytest
@@ -207,6 +215,8 @@ def test_append_outside_is_skipped():
 
 def check_attention(cache, qkv, hq, lengths, out, before):
     """`out` and `cache` after the call against `before`, the cache ahead of it."""
+    tiles = sum(n // 64 + 1 for n in lengths if 0 <= n < cache.max_seq) * cache.n_kv_heads
+    chain = 8 * (1 + tiles // 512)
     batch, hkv, dim, g = cache.batch, cache.n_kv_heads, cache.head_dim, hq // cache.n_kv_heads
     want = copy_of(before)
     q, k, v = qkv.split((hq * dim, hkv * dim, hkv * dim), dim=1)
@@ -219,9 +229,11 @@ def check_attention(cache, qkv, hq, lengths, out, before):
         for h in range(hkv):
             keys, values = content(want, b, h, n + 1)
             o, p, room, a = ref.attend(q[b].view(hkv, g, dim)[h].double(), keys, values)
-            off = 2 * 2.0 ** -18 * a + 2.0 ** -19
+            group_scale = want.k_scales[b, h, :n + 1].double().sum(-1).max() / math.sqrt(dim)
+            off = 2 * 2.0 ** -18 * a + 2 * 2.0 ** -10.9 * float(q[b].view(hkv, g, dim)[h].abs().max() * group_scale) + 2.0 ** -19
             err = (out[b].view(hkv, g, dim)[h].double() - o).abs()
-            tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18 + off) * room + 1e-30
+            ps = (p @ want.v_scales[b, h, :n + 1].double()).repeat_interleave(32, dim=1)
+            tol = 2.0 ** -8 * o.abs() + (2.0 ** -11 + 2.0 ** -18 + off) * room + (2.0 ** -10.9 + chain * 2.0 ** -18.4) * ps + 1e-30
             assert bool((err <= tol).all()), (b, h, n, float((err / tol).max()))
             if cache.weights is not None:
                 old = want.weights[b, h, :n + 1].double()
