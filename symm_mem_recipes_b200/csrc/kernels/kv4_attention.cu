@@ -94,6 +94,13 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with an accumulator that starts at (c0, c1) in both rows and is left as it is.
+__device__ __forceinline__ void mma_bf16_from(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
 __device__ __forceinline__ void mma_fp16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -230,9 +237,10 @@ struct Attend {
       }
 #pragma unroll
       for (int g = 0; g < kG; ++g) {
-        float d[4] = {minus8[g][0], minus8[g][1], minus8[g][0], minus8[g][1]};
+        float d[4];
         const uint32_t x = w[0][g], y = w[1][g];
-        mma_bf16(d, x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u, q[g][0][0], q[g][0][1]);
+        mma_bf16_from(d, minus8[g][0], minus8[g][1], x & 0x000F000Fu, y & 0x000F000Fu, x & 0x00F000F0u, y & 0x00F000F0u,
+                      q[g][0][0], q[g][0][1]);
         mma_bf16(d, x >> 8 & 0x000F000Fu, y >> 8 & 0x000F000Fu, x >> 8 & 0x00F000F0u, y >> 8 & 0x00F000F0u, q[g][1][0],
                  q[g][1][1]);
         const float sx = g & 1 ? hi_of(sc[0][g / 2]) : lo_of(sc[0][g / 2]);
@@ -242,14 +250,13 @@ struct Attend {
         s[sub][2] = g == 0 ? d[2] * sy : fmaf(d[2], sy, s[sub][2]);
         s[sub][3] = g == 0 ? d[3] * sy : fmaf(d[3], sy, s[sub][3]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[sub][i] *= to_log2[i & 1];
       if constexpr (kScores) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int row = sub * 16 + row_of(r) + 8 * j;
           if (2 * c < group && row < valid)
-            *reinterpret_cast<float2*>(scores + row * pitch + 2 * c) = make_float2(s[sub][2 * j], s[sub][2 * j + 1]);
+            *reinterpret_cast<float2*>(scores + row * pitch + 2 * c) =
+                make_float2(s[sub][2 * j] * to_log2[0], s[sub][2 * j + 1] * to_log2[1]);
         }
       }
     }
@@ -268,15 +275,23 @@ struct Attend {
         } else {
           sv[sub][j][0] = *reinterpret_cast<const uint32_t*>(ps);
         }
-        if (valid < kTile && row >= valid) {
-#pragma unroll
-          for (int i = 0; i < kG / 2; ++i) sv[sub][j][i] = 0;
-          s[sub][2 * j] = s[sub][2 * j + 1] = -INFINITY;
-        }
-#pragma unroll
-        for (int i = 0; i < kG / 2; ++i)      // of a NaN and a number this is the number
-          top2 = __hmax2(top2, *reinterpret_cast<const __nv_bfloat162*>(&sv[sub][j][i]));
       }
+    }
+    if (valid < kTile) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (i / 2 * 16 + row_of(r) + 8 * (i & 1) >= valid) {
+#pragma unroll
+          for (int k = 0; k < kG / 2; ++k) sv[i / 2][i & 1][k] = 0;
+          s[i / 2][2 * (i & 1)] = s[i / 2][2 * (i & 1) + 1] = -INFINITY;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int k = 0; k < kG / 2; ++k)      // of a NaN and a number this is the number
+        top2 = __hmax2(top2, *reinterpret_cast<const __nv_bfloat162*>(&sv[i / 2][i & 1][k]));
     }
     float top = fmaxf(__low2float(top2), __high2float(top2));
     float high[2];
@@ -292,7 +307,7 @@ struct Attend {
     }
     // 2^(e - 126) is above the largest scale; below 2^-60 it does not matter
     const float exponent = (float)(max((int)(__float_as_uint(top) >> 23), 66) - 126 - 15);
-    const float m0 = fmaxf(m[0], high[0] + exponent), m1 = fmaxf(m[1], high[1] + exponent);
+    const float m0 = fmaxf(m[0], fmaf(high[0], to_log2[0], exponent)), m1 = fmaxf(m[1], fmaf(high[1], to_log2[1], exponent));
     if (__any_sync(0xffffffffu, m0 != m[0] || m1 != m[1])) {
       const float f0 = exp2_of(m[0] - m0), f1 = exp2_of(m[1] - m1);
       m[0] = m0;
@@ -313,7 +328,7 @@ struct Attend {
     for (int sub = 0; sub < 4; ++sub) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        s[sub][i] = exp2_of(s[sub][i] - m[i & 1]);
+        s[sub][i] = exp2_of(fmaf(s[sub][i], to_log2[i & 1], -m[i & 1]));
         l[i & 1] += s[sub][i];
       }
     }
