@@ -6,8 +6,10 @@
 // infinity or a NaN gets a NaN scale, so that it reads back as NaN instead of as something plausible.
 //
 // Codes are exact whichever way the quotient is taken: x and s have 8-bit significands, so for |x| / s >= 1/2 the distance
-// of |x| / s from a half is 0 or at least 1 / 510 (2 |x| - (2 k + 1) s is a multiple of s's last bit).  |x| * (1 / s) is off
-// by 2^-22 of itself; times (1 - 2^-14) it is below the half for every exact half and on the right side for all else.
+// of |x| / s from a half is 0 or at least 1 / 510 (2 |x| - (2 k + 1) s is a multiple of s's last bit).  x * (1 / s) * (1 - 2^-14)
+// is off by 2^-22 of itself besides the factor: below the half for every exact half, on the right side for all else, and
+// never a half itself, so one fused multiply-add onto 1.5 * 2^23 + 8 rounds it and leaves the nibble in the low bits.  In the
+// same way a / 7 may be a * (1 / 7): 7 times a midpoint of two bf16 numbers is at least 2^-12 of itself away from any a.
 //
 // Order of the codes in a row.  Keys are an MMA operand whose lane c (of four) holds, group by group, eight neighbouring
 // dims of a key; values one whose lane r (of eight) holds four dims a group.  So
@@ -27,32 +29,35 @@ namespace kv4 {
 constexpr int kGroup = 32;
 constexpr int kTile = 64;        // a cache has a whole number of tiles of this many slots
 
-// Scale of a group whose largest magnitude is `a`, with the factor that x is multiplied by before it is rounded.
+// Scale of a group and the factor that x is multiplied by before it is rounded; `largest` is the largest magnitude's bits (an
+// infinity or a NaN counts as larger than any number).
 struct Scale {
-  __nv_bfloat16 s;
+  uint16_t bits;
+  bool finite;
   float inv;
 };
-__device__ __forceinline__ Scale scale_of(float a, bool finite) {
+__device__ __forceinline__ Scale scale_of(uint32_t largest) {
   Scale r;
-  if (!finite) {
-    r.s = __ushort_as_bfloat16((unsigned short)0x7FFF);
-    r.inv = 0.0f;
-  } else if (a < 7.888609052210118e-31f) {      // 2^-100
-    r.s = __ushort_as_bfloat16((unsigned short)0);
-    r.inv = 0.0f;
-  } else {
-    r.s = __float2bfloat16_rn(__fdiv_rn(a, 7.0f));
-    r.inv = __fmul_rn(__frcp_rn(__bfloat162float(r.s)), 0.99993896484375f);      // 1 - 2^-14
-  }
+  r.finite = largest < 0x7F80u;
+  const float a = __uint_as_float(largest << 16);
+  r.bits = __bfloat16_as_ushort(__float2bfloat16_rn(a * 0.14285714285714285f));
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(__uint_as_float((uint32_t)r.bits << 16)));
+  r.inv = inv * 0.99993896484375f;                      // 1 - 2^-14
+  if (largest < 0x0D80u) r.bits = 0, r.inv = 0.0f;      // 2^-100: held as zeros
+  if (!r.finite) r.bits = 0x7FFF;
   return r;
 }
-// Nibble of x under a scale; 8 (the value zero) under a scale of zero or NaN.
-__device__ __forceinline__ uint32_t nibble_of(float x, const Scale& s) {
-  if (s.inv == 0.0f) return 8;
-  const float steps = fminf(rintf(__fmul_rn(fabsf(x), s.inv)), 7.0f);
-  return (uint32_t)((int)(x < 0.0f ? -steps : steps) + 8);
+// 0x4B400000 + nibble of x under a finite scale.
+__device__ __forceinline__ uint32_t rounded(float x, const Scale& s) {
+  return __float_as_uint(fmaf(x, s.inv, 12582920.0f));
 }
-__device__ __forceinline__ bool is_finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+// Largest magnitude, as bits, of a pair of bf16 numbers and another two.
+__device__ __forceinline__ uint32_t max_magnitude(uint32_t x, uint32_t y) {
+  uint32_t r;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0x7FFF7FFFu), "r"(y & 0x7FFF7FFFu));
+  return r;
+}
 
 }  // namespace kv4
 }  // namespace smr

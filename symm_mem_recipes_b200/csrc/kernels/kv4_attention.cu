@@ -388,29 +388,22 @@ __device__ __forceinline__ void append_row(const Kv4AttentionArgs& a, int b, int
   for (int kind = 0; kind < 2; ++kind) {
     uint2 raw = make_uint2(0, 0);
     if (lane < D / 4) raw = *reinterpret_cast<const uint2*>(row + ((size_t)kind * hkv + h) * D + 4 * lane);
-    const float f[4] = {lo_of(raw.x), hi_of(raw.x), lo_of(raw.y), hi_of(raw.y)};
-    float largest = 0.0f;
-    bool finite = true;
+    uint32_t largest = max_magnitude(raw.x, raw.y);
+    largest = max(largest & 0xFFFFu, largest >> 16);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      finite = finite && is_finite(f[i]);
-      largest = fmaxf(largest, fabsf(f[i]));
-    }
-    if (!finite) largest = INFINITY;
-#pragma unroll
-    for (int o = 1; o <= 4; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    const Scale s = scale_of(largest, is_finite(largest));
-    uint32_t half = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) half |= nibble_of(f[i], s) << (4 * i);
+    for (int o = 1; o <= 4; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const Scale s = scale_of(largest);
+    uint32_t half = 0x4B400000u * 0xFFFFEEEFu;      // less 0x4B400000 in four nibbles' places
+    half += rounded(lo_of(raw.x), s) + (rounded(hi_of(raw.x), s) << 4) + (rounded(lo_of(raw.y), s) << 8) + (rounded(hi_of(raw.y), s) << 12);
+    if (!s.finite) half = 0x8888u;
     if (lane < D / 4) {
       const int byte = kind == 0 ? (lane & 7) / 2 * (D / 8) + g * 4 + (lane & 1) * 2 : (lane & 7) * (D / 16) + g * 2;
       uint8_t* codes = kind == 0 ? a.cache.k_codes : a.cache.v_codes;
       *reinterpret_cast<uint16_t*>(codes + at * (D / 2) + byte) = (uint16_t)half;
       *reinterpret_cast<uint16_t*>(stage + kind * L::kCodes + in_tile * (D / 2) + byte) = (uint16_t)half;
       if ((lane & 7) == 0) {
-        static_cast<__nv_bfloat16*>(kind == 0 ? a.cache.k_scales : a.cache.v_scales)[at * L::kGroups + g] = s.s;
-        reinterpret_cast<__nv_bfloat16*>(stage + 2 * L::kCodes + kind * L::kScales)[in_tile * L::kGroups + g] = s.s;
+        static_cast<uint16_t*>(kind == 0 ? a.cache.k_scales : a.cache.v_scales)[at * L::kGroups + g] = s.bits;
+        reinterpret_cast<uint16_t*>(stage + 2 * L::kCodes + kind * L::kScales)[in_tile * L::kGroups + g] = s.bits;
       }
     }
   }

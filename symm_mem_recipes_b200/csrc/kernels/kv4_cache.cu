@@ -51,22 +51,17 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Kv4
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
+    uint32_t largest = max_magnitude(max_magnitude(raw[u].x, raw[u].y), max_magnitude(raw[u].z, raw[u].w));
+    largest = max(largest & 0xFFFFu, largest >> 16);
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const Scale s = scale_of(largest);
     float f[8];
     unpack8(raw[u], f);
-    float largest = 0.0f;
-    bool finite = true;
+    uint32_t word = 0x4B400000u * 0xEEEEEEEFu;      // less 0x4B400000 in every nibble's place: 0x11111111 of them
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      finite = finite && is_finite(f[i]);
-      largest = fmaxf(largest, fabsf(f[i]));
-    }
-    if (!finite) largest = __uint_as_float(0x7F800000u);
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    const Scale s = scale_of(largest, is_finite(largest));
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) word |= nibble_of(f[i], s) << (4 * i);
+    for (int i = 0; i < 8; ++i) word += rounded(f[i], s) << (4 * i);
+    if (!s.finite) word = 0x88888888u;
     // a value row's part has two bytes a group: two lanes of neighbouring groups trade halves and write four bytes each
     const uint32_t other = __shfl_xor_sync(0xffffffffu, (g & 1) ? word & 0xFFFFu : word >> 16, 4);
     if (first + u * kStep >= rows) continue;
@@ -78,8 +73,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Kv4
       const uint32_t pair = (g & 1) ? other | (word & 0xFFFF0000u) : (word & 0xFFFFu) | (other << 16);
       *reinterpret_cast<uint32_t*>(codes + (2 * c + (g & 1)) * (D / 16) + (g >> 1) * 4) = pair;
     }
-    if (c == 0)
-      static_cast<__nv_bfloat16*>(is_value ? a.cache.v_scales : a.cache.k_scales)[at * (D / kGroup) + g] = s.s;
+    if (c == 0) static_cast<uint16_t*>(is_value ? a.cache.v_scales : a.cache.k_scales)[at * (D / kGroup) + g] = s.bits;
     if (l == 0 && !is_value && a.cache.weights != nullptr) a.cache.weights[at] = 0.0f;      // of the slot's last tenant
   }
 }
@@ -91,11 +85,11 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Ca
   const int l = threadIdx.x % kLanes, g = l >> 2, c = l & 3, b = blockIdx.y, hkv = cache.hkv, rows = n * hkv;
   const bool is_value = blockIdx.z != 0;
   const uint8_t* codes = (is_value ? cache.v_codes : cache.k_codes) + (is_value ? 2 * c * (D / 16) + g * 2 : c * (D / 8) + g * 4);
-  const __nv_bfloat16* scales = static_cast<const __nv_bfloat16*>(is_value ? cache.v_scales : cache.k_scales) + g;
+  const uint16_t* scales = static_cast<const uint16_t*>(is_value ? cache.v_scales : cache.k_scales) + g;
   __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_value ? v_out : k_out) + (size_t)b * rows * D + l * 8;
   const int first = blockIdx.x * (kStep * kRows) + threadIdx.x / kLanes;
   uint32_t word[kRows];
-  float s[kRows];
+  uint16_t s[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int i = first + u * kStep;
@@ -105,19 +99,23 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Ca
     const uint8_t* p = codes + at * (D / 2);
     word[u] = is_value ? *reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + D / 16) << 16
                        : *reinterpret_cast<const uint32_t*>(p);
-    s[u] = __bfloat162float(scales[at * (D / kGroup)]);
+    s[u] = scales[at * (D / kGroup)];
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const int i = first + u * kStep;
     if (i >= rows) continue;
-    float f[8];
+    // 128 + n as bf16, less 136, is exact; the product with the scale is rounded once
+    const __nv_bfloat162 scale = __bfloat162bfloat162(__ushort_as_bfloat16(s[u]));
+    uint32_t v[4];      // dims j and j + 4
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = s[u] * (float)((int)(word[u] >> (4 * k) & 15u) - 8);
-    Vec16 o;
-    o.x = pack_bf16x2(f[0], f[1]); o.y = pack_bf16x2(f[2], f[3]);
-    o.z = pack_bf16x2(f[4], f[5]); o.w = pack_bf16x2(f[6], f[7]);
-    st_16(out + (size_t)i * D, o);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t n = (word[u] >> (4 * j) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 x = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&n), __float2bfloat162_rn(136.0f)), scale);
+      v[j] = *reinterpret_cast<const uint32_t*>(&x);
+    }
+    st_16(out + (size_t)i * D, Vec16{__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                     __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)});
   }
 }
 
@@ -127,11 +125,12 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Ca
 //   1. a radix selection over the weights as ordered integers (kept in shared memory, so weights are read once) finds the
 //      weight of the last one kept, eight bits a pass; the CTAs' counts meet over distributed shared memory;
 //   2. warps count what stays of their own runs, the counts give every kept slot its place, and the places' sources are listed;
-//   3. rows move in chunks of places, 128 bytes and more a thread in registers.  A chunk is read whole before any of it
-//      is written; a place is never above its source and sources increase, so a chunk's writes cannot reach the sources of
-//      a later one.
-constexpr int kEvictThreads = 512;
+//   3. rows move in chunks of places, through shared memory by asynchronous copies (in registers 2048 rows of a cluster spilled
+//      and took 28 us of a prompt's 50).  A chunk is read whole before any of it is written; a place is never above its source
+//      and sources increase, so a chunk's writes cannot reach the sources of a later one.
+constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kEvictCtas = 8;          // of a cluster at most
 constexpr int kEvictKeys = 40960;      // weights of a CTA that stay in shared memory; beyond them they are read again
 
 // Order of a weight as an integer; NaN counts as an infinity; above all weights: the slots that stay anyway.
@@ -142,12 +141,33 @@ __device__ __forceinline__ uint32_t worth_of(float w, bool stays) {
   if (u == 0x80000000u) return u;                    // -0 and 0 are equal
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-__device__ __forceinline__ int load_remote(const int* local, int cta) {
-  uint32_t remote;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(cta));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
-  return v;
+template <int D>
+struct EvictRows {
+  static constexpr int kVecs = D / 32, kWords = D / 64;      // 16-byte parts of a row's codes, words of its scales
+  Vec16 codes[kEvictThreads * 2 * kVecs];
+  uint32_t scales[2][kEvictThreads][kWords];
+  float weights[kEvictThreads];
+};
+template <int N>
+__device__ __forceinline__ void copy_async(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(N) : "memory");
+}
+// Sum of an integer in shared memory over the cluster's first `ctas` CTAs; the loads are in flight together.
+__device__ __forceinline__ int sum_over_ctas(const int* local, int ctas) {
+  int v[kEvictCtas];
+#pragma unroll
+  for (int r = 0; r < kEvictCtas; ++r) {
+    v[r] = 0;
+    if (r < ctas) {
+      uint32_t remote;
+      asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_u32(local)), "r"(r));
+      asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[r]) : "r"(remote) : "memory");
+    }
+  }
+  int sum = 0;
+#pragma unroll
+  for (int r = 0; r < kEvictCtas; ++r) sum += v[r];
+  return sum;
 }
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -155,9 +175,9 @@ __device__ __forceinline__ void cluster_barrier() {
 }
 
 template <int D>
-__global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_constant__ Kv4EvictArgs a, int ctas, int cached) {
+__global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_constant__ Kv4EvictArgs a, int ctas, int cached) {
   pdl_wait();
-  extern __shared__ uint32_t keys[];                 // [cached]
+  extern __shared__ __align__(16) uint32_t keys[];   // [cached], then EvictRows
   __shared__ int hist[2][256];                       // two passes in turn: one barrier a pass
   __shared__ int total[256];
   __shared__ int counts[2];                          // of this CTA: slots above the last worth kept, slots equal to it
@@ -193,11 +213,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
     if (ctas > 1) cluster_barrier();
     else __syncthreads();
     if (tid < 256) {
-      int sum = 0;
-      if (ctas == 1) sum = bins[tid];
-      else
-        for (int r = 0; r < ctas; ++r) sum += load_remote(&bins[tid], r);
-      total[tid] = sum;
+      total[tid] = ctas == 1 ? bins[tid] : sum_over_ctas(&bins[tid], ctas);
       if (pass > 0) hist[(pass + 1) & 1][tid] = 0;   // the last pass's, which nobody reads any more
     }
     __syncthreads();
@@ -249,11 +265,7 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   if (ctas > 1) cluster_barrier();
   else __syncthreads();
   // slots above and equal in front of this warp's run
-  int above_before = 0, equal_before = 0;
-  for (int r = 0; r < cta; ++r) {
-    above_before += load_remote(&counts[0], r);
-    equal_before += load_remote(&counts[1], r);
-  }
+  int above_before = sum_over_ctas(&counts[0], cta), equal_before = sum_over_ctas(&counts[1], cta);
   for (int i = 0; i < warp; ++i) {
     above_before += warp_counts[0][i];
     equal_before += warp_counts[1][i];
@@ -273,49 +285,48 @@ __global__ void __launch_bounds__(kEvictThreads) evict_kernel(const __grid_const
   if (ctas > 1) cluster_barrier();      // the list is written, and nothing of another CTA's shared memory is read any more
   else __syncthreads();
 
-  constexpr int kVecs = D / 32, kParts = 2 * kVecs, kWords = D / 64;      // 16-byte parts of codes, words of scales a row
+  using Staged = EvictRows<D>;
+  constexpr int kVecs = Staged::kVecs, kParts = 2 * kVecs, kWords = Staged::kWords;
   Vec16* kc = reinterpret_cast<Vec16*>(a.cache.k_codes + base * (D / 2));
   Vec16* vc = reinterpret_cast<Vec16*>(a.cache.v_codes + base * (D / 2));
   uint32_t* ks = static_cast<uint32_t*>(a.cache.k_scales) + base * kWords;
   uint32_t* vs = static_cast<uint32_t*>(a.cache.v_scales) + base * kWords;
-  const int threads = ctas * kEvictThreads, me = cta * kEvictThreads + tid;
-  for (int first = 0; first < keep; first += threads) {      // a chunk: a row a thread, its codes spread over kParts threads
-    Vec16 x[kParts];
-    uint32_t scale[2 * kWords];
-    float weight = 0.0f;
+  Staged& rows = *reinterpret_cast<Staged*>(keys);   // the keys are done with
+  for (int chunk = 0; chunk < keep; chunk += ctas * kEvictThreads) {
+    const int first = chunk + cta * kEvictThreads;   // this CTA's places: a row a thread, its codes spread over kParts threads
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int item = i * threads + me, row = first + item / kParts, part = item % kParts;
+      const int item = i * kEvictThreads + tid, row = first + item / kParts, part = item % kParts;
       if (row < keep) {
         const size_t src = list[row];
-        x[i] = part < kVecs ? kc[src * kVecs + part] : vc[src * kVecs + part - kVecs];
+        copy_async<16>(&rows.codes[item], part < kVecs ? kc + src * kVecs + part : vc + src * kVecs + part - kVecs);
       }
     }
-    const int row = first + me;
-    if (row < keep) {
-      const size_t src = list[row];
-#pragma unroll
-      for (int i = 0; i < kWords; ++i) {
-        scale[i] = ks[src * kWords + i];
-        scale[kWords + i] = vs[src * kWords + i];
-      }
-      weight = w[src];
+    if (first + tid < keep) {
+      const size_t src = list[first + tid];
+      copy_async<4 * kWords>(rows.scales[0][tid], ks + src * kWords);
+      copy_async<4 * kWords>(rows.scales[1][tid], vs + src * kWords);
+      copy_async<4>(&rows.weights[tid], w + src);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (ctas > 1) cluster_barrier();
     else __syncthreads();
 #pragma unroll
     for (int i = 0; i < kParts; ++i) {
-      const int item = i * threads + me, to = first + item / kParts, part = item % kParts;
-      if (to < keep) (part < kVecs ? kc[(size_t)to * kVecs + part] : vc[(size_t)to * kVecs + part - kVecs]) = x[i];
+      const int item = i * kEvictThreads + tid, part = item % kParts;
+      const size_t to = first + item / kParts;
+      if (to < keep) *(part < kVecs ? kc + to * kVecs + part : vc + to * kVecs + part - kVecs) = rows.codes[item];
     }
-    if (row < keep) {
+    if (first + tid < keep) {
+      const size_t to = first + tid;
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
-        ks[(size_t)row * kWords + i] = scale[i];
-        vs[(size_t)row * kWords + i] = scale[kWords + i];
+        ks[to * kWords + i] = rows.scales[0][tid][i];
+        vs[to * kWords + i] = rows.scales[1][tid][i];
       }
-      w[row] = weight;
+      w[to] = rows.weights[tid];
     }
+    __syncthreads();      // the staged rows are written before the next ones come in
   }
 }
 
@@ -382,7 +393,7 @@ int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t stream) {
   const int ctas = a.cache.slots <= 1024 ? 1 : a.cache.slots <= 2048 ? 2 : a.cache.slots <= 4096 ? 4 : 8;
   const int run = ((a.cache.max_seq + ctas - 1) / ctas + kEvictThreads - 1) / kEvictThreads * kEvictThreads;
   const int cached = std::min(run, kEvictKeys);
-  const size_t smem = (size_t)cached * sizeof(uint32_t);
+  const size_t smem = std::max(cached * sizeof(uint32_t), a.cache.head_dim == 128 ? sizeof(EvictRows<128>) : sizeof(EvictRows<64>));
   auto kernel = a.cache.head_dim == 128 ? evict_kernel<128> : evict_kernel<64>;
   if (int e = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
   return launch_kernel(kernel, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), kEvictThreads, smem, ctas, stream, a, ctas, cached);
