@@ -22,35 +22,59 @@ __device__ __forceinline__ void unpack8(const Vec16& v, float (&f)[8]) {
   f[6] = bf16lo_to_f32(v.w); f[7] = bf16hi_to_f32(v.w);
 }
 
+// i / d for i < 2^30 by a multiplication: with s = 30 + ceil(log2 d) and m = 2^s / d rounded up, m * i / 2^s is above i / d by
+// less than i * d / (d * 2^s) <= 1 / d, which reaches no whole number; m <= 2^31 + 1, so m * i stays below 2^62.
+struct Divisor {
+  uint32_t d, step_div, step_mod;      // and of one number, the step from a thread's row to its next
+  uint32_t shift;
+  uint64_t m;
+  Divisor(uint32_t by, uint32_t step) : d(by), step_div(step / by), step_mod(step % by), shift(30) {
+    while (1ull << (shift - 30) < by) ++shift;
+    m = ((1ull << shift) + by - 1) / by;
+  }
+};
+// The row of a thread: token t, head h; kRows of them, a step apart.
+struct Row {
+  int t, h;
+  __device__ __forceinline__ Row(int i, const Divisor& by) : t((int)(by.m * (uint64_t)i >> by.shift)), h(i - t * (int)by.d) {}
+  __device__ __forceinline__ void next(const Divisor& by) {
+    t += by.step_div;
+    h += by.step_mod;
+    if (h >= (int)by.d) {
+      h -= by.d;
+      ++t;
+    }
+  }
+};
+
 // D / 8 lanes take a row of keys or of values, eight dims a lane, kRows rows a thread one after the other: their loads are in
 // flight together.  blockIdx.y is the sequence, blockIdx.z keys or values; row i of a sequence is head i % hkv of token i / hkv.
 // Memory-bound: 2 bytes a value on one side, 0.56 on the other.
-template <int D, int kRows>
-__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Kv4AppendArgs a) {
-  pdl_wait();
+template <int D, int kRows, bool kValue>
+__device__ __forceinline__ void append_rows(const Kv4AppendArgs& a, const Divisor& hkv) {
   constexpr int kLanes = D / 8, kStep = 256 / kLanes;
-  const int l = threadIdx.x % kLanes, g = l >> 2, c = l & 3, b = blockIdx.y, hkv = a.cache.hkv;
-  const bool is_value = blockIdx.z != 0;
-  const long long* stride = is_value ? a.v_stride : a.k_stride;
-  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(is_value ? a.v : a.k) + b * stride[0] + l * 8;
+  const int l = threadIdx.x % kLanes, g = l >> 2, c = l & 3, b = blockIdx.y;
+  const long long* stride = kValue ? a.v_stride : a.k_stride;
+  const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(kValue ? a.v : a.k) + b * stride[0] + l * 8;
   // `start` and `counts` may be any numbers: nothing is added to them before they are known to be slots
   const int start = a.start_dev ? a.start_dev[b] : a.start;
   int tokens = start >= 0 && start < a.cache.max_seq ? min(a.tokens, a.cache.max_seq - start) : 0;
   if (a.counts != nullptr) tokens = min(tokens, a.counts[b]);
-  const int rows = tokens > 0 ? tokens * hkv : 0;      // at most the sequence's slots in all heads
   const int first = blockIdx.x * (kStep * kRows) + threadIdx.x / kLanes;
   Vec16 raw[kRows];
-  int t[kRows], h[kRows];
+  Row row(first, hkv);
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const int i = first + u * kStep;
+  for (int u = 0; u < kRows; ++u, row.next(hkv)) {
     raw[u] = Vec16{0, 0, 0, 0};
-    t[u] = i / hkv;
-    h[u] = i - t[u] * hkv;
-    if (i < rows) raw[u] = ld_16_nc(src + t[u] * stride[1] + h[u] * stride[2]);
+    if (row.t < tokens) raw[u] = ld_16_nc(src + row.t * stride[1] + row.h * stride[2]);
   }
+  row = Row(first, hkv);
+  const size_t base = (size_t)b * hkv.d * a.cache.slots + max(start, 0);
+  // a value row's part has two bytes a group: two lanes of neighbouring groups trade halves and write four bytes each
+  uint8_t* codes = kValue ? a.cache.v_codes + (2 * c + (g & 1)) * (D / 16) + (g >> 1) * 4 : a.cache.k_codes + c * (D / 8) + g * 4;
+  uint16_t* scales = static_cast<uint16_t*>(kValue ? a.cache.v_scales : a.cache.k_scales) + g;
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
+  for (int u = 0; u < kRows; ++u, row.next(hkv)) {
     uint32_t largest = max_magnitude(max_magnitude(raw[u].x, raw[u].y), max_magnitude(raw[u].z, raw[u].w));
     largest = max(largest & 0xFFFFu, largest >> 16);
 #pragma unroll
@@ -62,61 +86,72 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Kv4
 #pragma unroll
     for (int i = 0; i < 8; ++i) word += rounded(f[i], s) << (4 * i);
     if (!s.finite) word = 0x88888888u;
-    // a value row's part has two bytes a group: two lanes of neighbouring groups trade halves and write four bytes each
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, (g & 1) ? word & 0xFFFFu : word >> 16, 4);
-    if (first + u * kStep >= rows) continue;
-    const size_t at = ((size_t)b * hkv + h[u]) * a.cache.slots + start + t[u];
-    uint8_t* codes = (is_value ? a.cache.v_codes : a.cache.k_codes) + at * (D / 2);
-    if (!is_value) {
-      *reinterpret_cast<uint32_t*>(codes + c * (D / 8) + g * 4) = word;
-    } else {
-      const uint32_t pair = (g & 1) ? other | (word & 0xFFFF0000u) : (word & 0xFFFFu) | (other << 16);
-      *reinterpret_cast<uint32_t*>(codes + (2 * c + (g & 1)) * (D / 16) + (g >> 1) * 4) = pair;
+    if (kValue) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, __byte_perm(word, 0, (g & 1) ? 0x5410 : 0x7632), 4);
+      word = __byte_perm(word, other, (g & 1) ? 0x3254 : 0x5410);
     }
-    if (c == 0) static_cast<uint16_t*>(is_value ? a.cache.v_scales : a.cache.k_scales)[at * (D / kGroup) + g] = s.bits;
-    if (l == 0 && !is_value && a.cache.weights != nullptr) a.cache.weights[at] = 0.0f;      // of the slot's last tenant
+    if (row.t < tokens) {
+      const size_t at = base + (size_t)row.h * a.cache.slots + row.t;
+      *reinterpret_cast<uint32_t*>(codes + at * (D / 2)) = word;
+      if (c == 0) scales[at * (D / kGroup)] = s.bits;
+      if (!kValue && l == 0 && a.cache.weights != nullptr) a.cache.weights[at] = 0.0f;      // of the slot's last tenant
+    }
   }
 }
-
 template <int D, int kRows>
-__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Cache cache, int n, void* k_out, void* v_out) {
+__global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ Kv4AppendArgs a, const __grid_constant__ Divisor hkv) {
   pdl_wait();
+  if (blockIdx.z == 0) append_rows<D, kRows, false>(a, hkv);
+  else append_rows<D, kRows, true>(a, hkv);
+}
+
+template <int D, int kRows, bool kValue>
+__device__ __forceinline__ void read_rows(const Kv4Cache& cache, const Divisor& hkv, int n, void* to) {
   constexpr int kLanes = D / 8, kStep = 256 / kLanes;
-  const int l = threadIdx.x % kLanes, g = l >> 2, c = l & 3, b = blockIdx.y, hkv = cache.hkv, rows = n * hkv;
-  const bool is_value = blockIdx.z != 0;
-  const uint8_t* codes = (is_value ? cache.v_codes : cache.k_codes) + (is_value ? 2 * c * (D / 16) + g * 2 : c * (D / 8) + g * 4);
-  const uint16_t* scales = static_cast<const uint16_t*>(is_value ? cache.v_scales : cache.k_scales) + g;
-  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(is_value ? v_out : k_out) + (size_t)b * rows * D + l * 8;
+  const int l = threadIdx.x % kLanes, g = l >> 2, c = l & 3, b = blockIdx.y;
+  const uint8_t* codes = kValue ? cache.v_codes + 2 * c * (D / 16) + g * 2 : cache.k_codes + c * (D / 8) + g * 4;
+  const uint16_t* scales = static_cast<const uint16_t*>(kValue ? cache.v_scales : cache.k_scales) + g;
   const int first = blockIdx.x * (kStep * kRows) + threadIdx.x / kLanes;
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(to) + ((size_t)b * n * hkv.d + first) * D + l * 8;
+  const size_t base = (size_t)b * hkv.d * cache.slots;
   uint32_t word[kRows];
   uint16_t s[kRows];
+  Row row(first, hkv);
+  int rows = 0;
 #pragma unroll
-  for (int u = 0; u < kRows; ++u) {
-    const int i = first + u * kStep;
-    if (i >= rows) continue;
-    const int t = i / hkv, h = i - t * hkv;
-    const size_t at = ((size_t)b * hkv + h) * cache.slots + t;
-    const uint8_t* p = codes + at * (D / 2);
-    word[u] = is_value ? *reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + D / 16) << 16
+  for (int u = 0; u < kRows; ++u, row.next(hkv)) {
+    word[u] = s[u] = 0;
+    if (row.t < n) {
+      rows = u + 1;
+      const size_t at = base + (size_t)row.h * cache.slots + row.t;
+      const uint8_t* p = codes + at * (D / 2);
+      word[u] = kValue ? *reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + D / 16) << 16
                        : *reinterpret_cast<const uint32_t*>(p);
-    s[u] = scales[at * (D / kGroup)];
+      s[u] = scales[at * (D / kGroup)];
+    }
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
-    const int i = first + u * kStep;
-    if (i >= rows) continue;
+    if (u >= rows) break;
     // 128 + n as bf16, less 136, is exact; the product with the scale is rounded once
     const __nv_bfloat162 scale = __bfloat162bfloat162(__ushort_as_bfloat16(s[u]));
     uint32_t v[4];      // dims j and j + 4
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t n = (word[u] >> (4 * j) & 0x000F000Fu) | 0x43004300u;
-      const __nv_bfloat162 x = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&n), __float2bfloat162_rn(136.0f)), scale);
+      const uint32_t n4 = (word[u] >> (4 * j) & 0x000F000Fu) | 0x43004300u;
+      const __nv_bfloat162 x = __hmul2(__hsub2(*reinterpret_cast<const __nv_bfloat162*>(&n4), __float2bfloat162_rn(136.0f)), scale);
       v[j] = *reinterpret_cast<const uint32_t*>(&x);
     }
-    st_16(out + (size_t)i * D, Vec16{__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
-                                     __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)});
+    st_16(out + (size_t)u * kStep * D, Vec16{__byte_perm(v[0], v[1], 0x5410), __byte_perm(v[2], v[3], 0x5410),
+                                             __byte_perm(v[0], v[1], 0x7632), __byte_perm(v[2], v[3], 0x7632)});
   }
+}
+template <int D, int kRows>
+__global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Cache cache, const __grid_constant__ Divisor hkv, int n,
+                                                   void* k_out, void* v_out) {
+  pdl_wait();
+  if (blockIdx.z == 0) read_rows<D, kRows, false>(cache, hkv, n, k_out);
+  else read_rows<D, kRows, true>(cache, hkv, n, v_out);
 }
 
 // ---- eviction ----
@@ -358,14 +393,15 @@ bool many_rows(long long rows, int batch, int head_dim) {
 template <int D, int kRows>
 int append(const Kv4AppendArgs& a, long long rows, cudaStream_t stream) {
   constexpr int kBlock = 256 / (D / 8) * kRows;
-  return launch_kernel(append_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), a.batch, 2), 256, 0, 1, stream, a);
+  return launch_kernel(append_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), a.batch, 2), 256, 0, 1, stream, a,
+                       Divisor(a.cache.hkv, 256 / (D / 8)));
 }
 template <int D, int kRows>
 int read(const Kv4Cache& cache, int batch, int n, void* k_out, void* v_out, cudaStream_t stream) {
   constexpr int kBlock = 256 / (D / 8) * kRows;
   const long long rows = (long long)n * cache.hkv;
-  return launch_kernel(read_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), batch, 2), 256, 0, 1, stream, cache, n,
-                       k_out, v_out);
+  return launch_kernel(read_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), batch, 2), 256, 0, 1, stream, cache,
+                       Divisor(cache.hkv, 256 / (D / 8)), n, k_out, v_out);
 }
 
 }  // namespace
