@@ -1348,9 +1348,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     a.length = (int)length;
     a.lengths = int_ptr(lengths);
     a.num_sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-    torch::Tensor workspace = new_tensor({(int64_t)kv4_attention_workspace_bytes(a.cache, a.batch, a.group, a.num_sms)},
-                                         torch::kUInt8, dev);
-    a.workspace = workspace.data_ptr();
+    torch::Tensor workspace;
+    if (const size_t bytes = kv4_attention_workspace_bytes(a.cache, a.batch, a.group, a.num_sms)) {
+      workspace = new_tensor({(int64_t)bytes}, torch::kUInt8, dev);
+      a.workspace = workspace.data_ptr();
+    }
     rt_check(launch_kv4_attention(a, current_stream(dev)), "kv4_decode_attention");
     return o;
   }, py::arg("qkv"), py::arg("k_codes"), py::arg("k_scales"), py::arg("v_codes"), py::arg("v_scales"), py::arg("weights"),

@@ -367,6 +367,21 @@ struct Attend {
     return make_float4(fmaf(acc[g][0][j], kEven, -e), fmaf(acc[g][0][2 + j], kOdd, -e), fmaf(acc[g][1][j], kEven, -e),
                        fmaf(acc[g][1][2 + j], kOdd, -e));
   }
+  // The piece: maxima, sums (after join_lanes), weighted values.
+  __device__ __forceinline__ void leave(float* piece, int group) const {
+    const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int head = 2 * c + j;
+      if (head >= group) continue;
+      if (r == 0) {
+        piece[head] = m[j];
+        piece[kHeads + head] = l[j];
+      }
+#pragma unroll
+      for (int g = 0; g < kG; ++g) *reinterpret_cast<float4*>(piece + 2 * kHeads + head * D + kGroup * g + 4 * r) = values(g, j);
+    }
+  }
   __device__ __forceinline__ void join_lanes() {
 #pragma unroll
     for (int o = 4; o <= 16; o <<= 1) {
@@ -406,6 +421,29 @@ __device__ __forceinline__ void append_row(const Kv4AttentionArgs& a, int b, int
         reinterpret_cast<uint16_t*>(stage + 2 * L::kCodes + kind * L::kScales)[in_tile * L::kGroups + g] = s.bits;
       }
     }
+  }
+}
+
+// A warp's copy of the tile that starts at row `slot` (of all heads) into a stage of its ring.
+template <int D>
+__device__ __forceinline__ void fetch_tile(const Kv4Cache& cache, size_t slot, uint32_t stage) {
+  using L = Layout<D>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t dst = stage + lane * 16;
+  const uint8_t* kc = cache.k_codes + slot * (D / 2) + lane * 16;
+  const uint8_t* vc = cache.v_codes + slot * (D / 2) + lane * 16;
+#pragma unroll
+  for (int i = 0; i < L::kCodes / 512; ++i) {
+    copy_async_16(dst + i * 512, kc + i * 512);
+    copy_async_16(dst + L::kCodes + i * 512, vc + i * 512);
+  }
+  const uint8_t* ks = static_cast<const uint8_t*>(cache.k_scales) + slot * (2 * L::kGroups);
+  const uint8_t* vs = static_cast<const uint8_t*>(cache.v_scales) + slot * (2 * L::kGroups);
+  if constexpr (D == 128) {
+    copy_async_16(dst + 2 * L::kCodes, ks + lane * 16);
+    copy_async_16(dst + 2 * L::kCodes + L::kScales, vs + lane * 16);
+  } else {      // 256 bytes of either, half a warp each
+    copy_async_16(dst + 2 * L::kCodes, lane < 16 ? ks + lane * 16 : vs + (lane - 16) * 16);
   }
 }
 
@@ -472,23 +510,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   uint8_t* ring = smem + warp * kRing;
   const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
   auto fetch = [&](const Cursor& at, int stage) {
-    const size_t slot = ((size_t)at.b * hkv + at.h) * a.cache.slots + (size_t)at.t * kTile;
-    const uint32_t dst = ring_addr + stage * L::kBytes + lane * 16;
-    const uint8_t* kc = a.cache.k_codes + slot * (D / 2) + lane * 16;
-    const uint8_t* vc = a.cache.v_codes + slot * (D / 2) + lane * 16;
-#pragma unroll
-    for (int i = 0; i < L::kCodes / 512; ++i) {
-      copy_async_16(dst + i * 512, kc + i * 512);
-      copy_async_16(dst + L::kCodes + i * 512, vc + i * 512);
-    }
-    const uint8_t* ks = static_cast<const uint8_t*>(a.cache.k_scales) + slot * (2 * L::kGroups);
-    const uint8_t* vs = static_cast<const uint8_t*>(a.cache.v_scales) + slot * (2 * L::kGroups);
-    if constexpr (D == 128) {
-      copy_async_16(dst + 2 * L::kCodes, ks + lane * 16);
-      copy_async_16(dst + 2 * L::kCodes + L::kScales, vs + lane * 16);
-    } else {      // 256 bytes of either, half a warp each
-      copy_async_16(dst + 2 * L::kCodes, lane < 16 ? ks + lane * 16 : vs + (lane - 16) * 16);
-    }
+    fetch_tile<D>(a.cache, ((size_t)at.b * hkv + at.h) * a.cache.slots + (size_t)at.t * kTile, ring_addr + stage * L::kBytes);
   };
   Cursor ahead = now;
   int to_fetch = first;
@@ -529,14 +551,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     stage = stage == L::kStages - 1 ? 0 : stage + 1;
     if (last || i + 1 == end) {
       at.join_lanes();
-      const int r = lane >> 2, c = lane & 3;
       const bool finished = last && whole;
-      float* piece = ws.pieces + ((size_t)w * 2 + (first_head ? 0 : 1)) * L::kPiece;
+      if (finished) {
+        const int r = lane >> 2, c = lane & 3;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int head = 2 * c + j;
-        if (head >= a.group) continue;
-        if (finished) {
+        for (int j = 0; j < 2; ++j) {
+          const int head = 2 * c + j;
+          if (head >= a.group) continue;
           const float inv = 1.0f / at.l[j];
           __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (((size_t)now.b * hkv + now.h) * a.group + head) * D + 4 * r;
 #pragma unroll
@@ -547,15 +568,9 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
           }
           if (kScores && r == 0)
             ws.stats[((size_t)now.b * hkv + now.h) * kHeads + head] = make_float2(at.m[j], at.l[j]);
-        } else {
-          if (r == 0) {
-            piece[head] = at.m[j];
-            piece[kHeads + head] = at.l[j];
-          }
-#pragma unroll
-          for (int g = 0; g < L::kGroups; ++g)
-            *reinterpret_cast<float4*>(piece + 2 * kHeads + head * D + kGroup * g + 4 * r) = at.values(g, j);
         }
+      } else {
+        at.leave(ws.pieces + ((size_t)w * 2 + (first_head ? 0 : 1)) * L::kPiece, a.group);
       }
       first_head = false;
       whole = true;
@@ -667,7 +682,21 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return;
   }
   if constexpr (kScores) {
-    const int q = tid % kHeads;
+    // what this thread accumulates comes in while the heads' maxima and sums are found
+    constexpr int kMine = kJoinTiles * kTile / kJoinThreads;
+    const int q = tid % kHeads, pitch = padded_group(a.group), len = length_of(a, b), i0 = chunk * kJoinTiles * kTile + tid;
+    const float* scores = ws.scores + (size_t)s0 * kTile * pitch;
+    float2 x[kMine][kHeads / 2];
+    float weight[kMine];
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = i0 + k * kJoinThreads;
+      if (i > len) continue;
+      weight[k] = a.cache.weights[(size_t)bh * a.cache.slots + i];
+#pragma unroll
+      for (int j = 0; j < kHeads / 2; ++j)
+        if (2 * j < a.group) x[k][j] = *reinterpret_cast<const float2*>(scores + (size_t)i * pitch + 2 * j);
+    }
     if (wa == wb) {
       if (tid < kHeads && q < a.group) {
         const float2 s = ws.stats[(size_t)bh * kHeads + q];
@@ -706,21 +735,206 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       }
     }
     __syncthreads();
-    const int pitch = padded_group(a.group), len = length_of(a, b);
-    const int end = min(len + 1, (chunk + 1) * kJoinTiles * kTile);
     float* weights = a.cache.weights + (size_t)bh * a.cache.slots;
-    const float* scores = ws.scores + (size_t)s0 * kTile * pitch;
-    for (int i = chunk * kJoinTiles * kTile + tid; i < end; i += kJoinThreads) {
-      const float2* s = reinterpret_cast<const float2*>(scores + (size_t)i * pitch);
+#pragma unroll
+    for (int k = 0; k < kMine; ++k) {
+      const int i = i0 + k * kJoinThreads;
+      if (i > len) continue;
       float p = 0.0f;
-      for (int j = 0; j < a.group; j += 2) {
-        const float2 x = s[j / 2];
-        p += exp2_of(x.x - norms[0][j]) * norms[1][j];
-        if (j + 1 < a.group) p += exp2_of(x.y - norms[0][j + 1]) * norms[1][j + 1];
+#pragma unroll
+      for (int j = 0; j < kHeads / 2; ++j) {
+        if (2 * j < a.group) p += exp2_of(x[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
+        if (2 * j + 1 < a.group) p += exp2_of(x[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
       }
-      weights[i] = i == len ? p : weights[i] + p;
+      weights[i] = i == len ? p : weight[k] + p;
     }
   }
+}
+
+// ---- one launch for caches of up to 2048 slots a head and CTA ----
+// A cluster of C CTAs takes a head, tile i the warp i % (8 C).  The warps' pieces meet in shared memory, the CTAs' over
+// distributed shared memory, and the scores wait in shared memory for their maxima and sums: no scratch, no second kernel.
+// 16 heads of up to 8192 with weights: 22.9 us as two launches.
+constexpr int kHeadWarps = 8;
+constexpr int kHeadTiles = 4;        // of a warp at most
+constexpr int kHeadStages = 2;
+constexpr int kHeadCtas = 8;
+
+__device__ __forceinline__ uint32_t remote_of(const void* local, int cta) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(local)), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ float load_remote(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load_remote_4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Joins `n` pieces of one head into (m, l, four dims); `get(i, what)`: what = 0 the maximum, 1 the sum, and get4(i) the dims.  A
+// piece that saw no tile has a maximum of minus infinity and zeros; one whose scores were all NaN has the same maximum and
+// a sum of NaN, which stays one.
+template <int N, class Get, class Get4>
+__device__ __forceinline__ void join_pieces(int n, Get get, Get4 get4, float& m, float& l, float4& o) {
+  float mi[N], li[N];
+  float4 oi[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mi[i] = i < n ? get(i, 0) : -INFINITY;
+    li[i] = i < n ? get(i, 1) : 0.0f;
+    oi[i] = i < n ? get4(i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  m = mi[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, mi[i]);
+  l = 0.0f;
+  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = mi[i] == -INFINITY ? 0.0f : exp2_of(mi[i] - m);
+    l += f * li[i];
+    o.x += f * oi[i].x; o.y += f * oi[i].y; o.z += f * oi[i].z; o.w += f * oi[i].w;
+  }
+}
+
+template <int D, bool kScores>
+__global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const __grid_constant__ Kv4AttentionArgs a, int ctas,
+                                                                         int tiles_a_warp) {
+  using L = Layout<D>;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(16) float cta_piece[L::kPiece];
+  __shared__ float norms[2][kHeads];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, tid = threadIdx.x, hkv = a.cache.hkv;
+  const int bh = blockIdx.x / ctas, rank = blockIdx.x % ctas, b = bh / hkv, h = bh % hkv;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int len = length_of(a, b);
+  __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (size_t)bh * a.group * D;
+  if (len < 0 || len >= a.cache.max_seq) {      // idle, for the whole cluster
+    for (int i = tid; rank == 0 && i < a.group * D / 8; i += 32 * kHeadWarps) st_16(out + 8 * i, Vec16{0, 0, 0, 0});
+    return;
+  }
+  const int n = len / kTile + 1, step = kHeadWarps * ctas, first = rank * kHeadWarps + warp, pitch = padded_group(a.group);
+  const int score_bytes = kScores ? tiles_a_warp * kTile * pitch * (int)sizeof(float) : 0;
+  uint8_t* ring = smem + warp * (kHeadStages * L::kBytes + score_bytes);
+  float* scores = reinterpret_cast<float*>(ring + kHeadStages * L::kBytes);      // [tile][kTile][pitch]
+  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+  const size_t base = (size_t)bh * a.cache.slots;
+#pragma unroll
+  for (int i = 0; i < kHeadStages; ++i) {
+    const int t = first + i * step;
+    if (t < n) fetch_tile<D>(a.cache, base + (size_t)t * kTile, ring_addr + i * L::kBytes);
+    copy_commit();
+  }
+  Attend<D, kScores> at;
+  at.start(a, b, h);
+  for (int t = first, i = 0; t < n; t += step, ++i) {
+    copy_wait<kHeadStages - 1>();
+    __syncwarp();
+    uint8_t* stage = ring + (i % kHeadStages) * L::kBytes;
+    int valid = kTile;
+    if (t == n - 1) {
+      valid = len % kTile + 1;
+      append_row<D>(a, b, h, len, stage);
+      __syncwarp();
+    }
+    at.tile(stage, valid, scores + i * kTile * pitch, a.group, pitch);
+    __syncwarp();
+    const int next = t + kHeadStages * step;
+    if (next < n) fetch_tile<D>(a.cache, base + (size_t)next * kTile, ring_addr + (i % kHeadStages) * L::kBytes);
+    copy_commit();
+  }
+  copy_wait<0>();
+  __syncwarp();
+  at.join_lanes();
+  at.leave(reinterpret_cast<float*>(ring), a.group);      // where the tiles were
+  __syncthreads();
+  constexpr int kSide = D / 4;                            // threads a query head, four dims each
+  const int side = tid / kSide, d = tid % kSide;
+  float m, l;
+  float4 o;
+  if (side < a.group) {
+    join_pieces<kHeadWarps>(
+        kHeadWarps,
+        [&](int i, int what) {
+          return reinterpret_cast<const float*>(smem + i * (kHeadStages * L::kBytes + score_bytes))[what * kHeads + side];
+        },
+        [&](int i) {
+          return reinterpret_cast<const float4*>(smem + i * (kHeadStages * L::kBytes + score_bytes))[(2 * kHeads + side * D) / 4 + d];
+        },
+        m, l, o);
+    if (d == 0) {
+      cta_piece[side] = m;
+      cta_piece[kHeads + side] = l;
+    }
+    reinterpret_cast<float4*>(cta_piece)[(2 * kHeads + side * D) / 4 + d] = o;
+  }
+  int q = side;
+  bool mine = side < a.group;
+  __syncwarp();
+  if (ctas > 1) {
+    cluster_arrive();
+    cluster_wait();
+    q = rank + side * ctas;      // query heads are dealt to the CTAs
+    mine = q < a.group;
+    if (mine)
+      join_pieces<kHeadCtas>(
+          ctas, [&](int i, int what) { return load_remote(remote_of(cta_piece + what * kHeads + q, i)); },
+          [&](int i) { return load_remote_4(remote_of(cta_piece + 2 * kHeads + q * D + 4 * d, i)); }, m, l, o);
+  }
+  if (mine) {
+    const float inv = 1.0f / l;
+    *reinterpret_cast<uint2*>(out + q * D + 4 * d) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  }
+  if constexpr (kScores) {
+    if (tid < a.group) {
+      float4 none;
+      if (ctas > 1)
+        join_pieces<kHeadCtas>(
+            ctas, [&](int i, int what) { return load_remote(remote_of(cta_piece + what * kHeads + tid, i)); },
+            [&](int) { return make_float4(0.0f, 0.0f, 0.0f, 0.0f); }, m, l, none);
+      else
+        m = cta_piece[tid], l = cta_piece[kHeads + tid];
+      norms[0][tid] = m;
+      norms[1][tid] = 1.0f / l;
+    }
+  }
+  __syncwarp();
+  if (ctas > 1) cluster_arrive();      // nothing of another CTA's is read from here on
+  if constexpr (kScores) {
+    __syncthreads();
+    float* weights = a.cache.weights + base;
+    for (int t = first, i = 0; t < n; t += step, ++i) {
+#pragma unroll
+      for (int k = 0; k < kTile / 32; ++k) {
+        const int slot = t * kTile + k * 32 + lane;
+        if (slot > len) continue;
+        const float* s = scores + (i * kTile + k * 32 + lane) * pitch;
+        float p = 0.0f;
+        for (int j = 0; j < a.group; ++j) p += exp2_of(s[j] - norms[0][j]) * norms[1][j];
+        weights[slot] = slot == len ? p : weights[slot] + p;
+      }
+    }
+  }
+  __syncwarp();
+  if (ctas > 1) cluster_wait();
+}
+
+// CTAs a head of the kernel above, or 0 where it does not take the call: heads of more slots than it has room for, or more heads
+// than a wave of CTAs (148 SMs hold sixteen clusters of eight).
+int head_ctas(const Kv4Cache& cache, int batch, int num_sms) {
+  const long long heads = (long long)batch * cache.hkv;
+  const int tiles = cache.slots / kTile;
+  int ctas = 1;
+  while (ctas < kHeadCtas && 2 * ctas * heads * 8 <= 7ll * num_sms && ctas * kHeadWarps < tiles) ctas *= 2;
+  return heads <= num_sms && tiles <= ctas * kHeadWarps * kHeadTiles ? ctas : 0;
 }
 
 int attention_ctas(const Kv4Cache& cache, int batch, int num_sms) {
@@ -728,34 +942,48 @@ int attention_ctas(const Kv4Cache& cache, int batch, int num_sms) {
   return (int)std::max<long long>(1, std::min<long long>(2ll * num_sms, (tiles + kWarps - 1) / kWarps));
 }
 
-template <int D, bool kScores>
-int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
-  const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
-  const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
-  int e = (int)cudaFuncSetAttribute(attend_kernel<D, kScores>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != 0) return e;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
+template <class... Params, class... Args>
+int launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
+  if (smem > 0)
+    if (int e = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
+  cudaLaunchAttribute attrs[2] = {};
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(32 * kWarps);
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  e = (int)cudaLaunchKernelEx(&cfg, attend_kernel<D, kScores>, a);
-  if (e != 0) return e;
-  const int chunks = kScores ? (a.cache.slots / kTile + kJoinTiles - 1) / kJoinTiles : 0;
-  cfg.gridDim = dim3(a.batch * a.cache.hkv, a.group + chunks);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.dynamicSmemBytes = 0;
-  return (int)cudaLaunchKernelEx(&cfg, join_kernel<D, kScores>, a, ctas * kWarps);
+  cfg.attrs = attrs;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+template <int D, bool kScores>
+int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
+  const int tiles = a.cache.slots / kTile;
+  if (const int ctas = head_ctas(a.cache, a.batch, a.num_sms)) {
+    const int a_warp = std::max(1, (tiles + ctas * kHeadWarps - 1) / (ctas * kHeadWarps));
+    const size_t smem = kHeadWarps * ((size_t)kHeadStages * Layout<D>::kBytes +
+                                      (kScores ? (size_t)a_warp * kTile * padded_group(a.group) * sizeof(float) : 0));
+    return launch_kernel(attend_head_kernel<D, kScores>, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), 32 * kHeadWarps, smem, ctas,
+                         stream, a, ctas, a_warp);
+  }
+  const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
+  const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
+  if (int e = launch_kernel(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
+  const int chunks = kScores ? (tiles + kJoinTiles - 1) / kJoinTiles : 0;
+  return launch_kernel(join_kernel<D, kScores>, dim3(a.batch * a.cache.hkv, a.group + chunks), kJoinThreads, 0, 1, stream, a,
+                       ctas * kWarps);
 }
 
 }  // namespace
 
 size_t kv4_attention_workspace_bytes(const Kv4Cache& cache, int batch, int group, int num_sms) {
+  if (head_ctas(cache, batch, num_sms) > 0) return 0;
   const size_t warps = (size_t)attention_ctas(cache, batch, num_sms) * kWarps;
   size_t bytes = warps * 2 * kHeads * (cache.head_dim + 2) * sizeof(float) + (size_t)batch * cache.hkv * kHeads * sizeof(float2);
   if (cache.weights != nullptr) bytes += (size_t)batch * cache.hkv * cache.slots * padded_group(group) * sizeof(float);

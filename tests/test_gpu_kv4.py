@@ -262,6 +262,7 @@ def test_decode_attention(dim, hkv, g, weights, lengths):
 
 @pytest.mark.parametrize("batch, hkv, g, dim, max_seq, least", [
     (1, 1, 8, 128, 20011, 20010), (2, 2, 4, 128, 9001, 1), (40, 2, 3, 64, 700, 0), (300, 1, 2, 64, 100, 0), (1, 8, 8, 64, 33000, 32000),
+    (160, 1, 8, 128, 130, -9), (75, 2, 5, 128, 320, -40), (19, 8, 1, 64, 1000, 0), (3, 3, 7, 128, 5000, 0), (33, 2, 8, 128, 2048, 0),
 ])
 def test_decode_attention_long_and_many(batch, hkv, g, dim, max_seq, least):
     """Contexts over many tiles and CTAs, batches over many warps, ragged lengths."""
