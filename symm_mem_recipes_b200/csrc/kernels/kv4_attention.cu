@@ -3,16 +3,17 @@
 //
 // The work is the caches' bytes.  Tiles of 64 slots of all heads and sequences form one list, cut evenly among the grid's
 // warps whatever the lengths are; a warp streams its tiles through a ring in shared memory by asynchronous copies and
-// nothing synchronises warps.  A head whose tiles are all one warp's is finished there, the others leave a piece (maximum,
-// sum, weighted values) per warp, which a second kernel joins in the warps' order: results do not depend on timing.
+// nothing synchronises warps until the end.  A head whose tiles are all one CTA's is finished there, the others leave a piece
+// (maximum, sum, weighted values) a CTA, which a second kernel joins in the CTAs' order: results do not depend on timing.
 //
 // Codes are multiplied as they are.  A nibble in the low bits of a 16-bit float is the subnormal n * 2^-133 (bf16), one in
 // the next four bits sixteen times that, and the tensor cores take subnormals exactly and at full rate (2.4 cycles an
 // MMA and SM, as normal numbers): one AND makes two operands, where a conversion would take three instructions.  Of
 // n = c + 8 the eight is taken out of the sums: in S by an accumulator that starts at -8 sum(q), in the values by one
-// more MMA a group that sums P'.  The cores align addends by their nominal exponents, a subnormal's being 2^-14 (fp16)
+// more MMA a group whose operand is eight everywhere.  The cores align addends by their nominal exponents, a subnormal's being 2^-14 (fp16)
 // however small it is: in the lowest bits a nibble would lose ten bits of the sum's 24.  fp16 nibbles therefore stand two bits
-// higher, where the lower one loses six at most, the upper two.
+// higher, where the lower one loses six at most, the upper two, and what is cut off the sums of eights in the same places
+// takes the bias out.
 //
 //   S^T [16 keys x 8 heads] = K q^T, bf16: q is exact, scaled by a power of two per head so that its largest element is
 //   near 2^120; a group's 32 dims are two MMAs, whose sum the key's scale multiplies in fp32.  No operand is rounded.
@@ -40,7 +41,7 @@ constexpr int kWarps = 4;                 // of an attention CTA
 constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
 constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
 constexpr int kJoinThreads = 256;
-constexpr int kJoinTiles = 16;            // tiles whose weights one CTA of the second kernel accumulates
+constexpr int kJoinTiles = 16;            // tiles whose weights a CTA of the second kernel accumulates at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -125,6 +126,14 @@ __device__ __forceinline__ float exp2_of(float x) {
 __device__ __forceinline__ float lo_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 << 16); }
 __device__ __forceinline__ float hi_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 & 0xFFFF0000u); }
 
+// What a warp of the list ends with: a head that it does not finish by itself (sequence * kv heads + kv head).
+struct FinalPiece {
+  int head;
+  bool whole, last;      // has the head's first tile, its last one
+  int slot;              // of its two pieces' places
+};
+constexpr int kNoPiece = -1, kNoTiles = -2;
+
 // Where a warp is in the list of tiles.
 struct Cursor {
   int b, h, t, n;      // sequence, kv head, tile of it, tiles of the head
@@ -146,7 +155,7 @@ struct Attend {
   float to_log2[2];         // S in the accumulators' units -> units of log2
   float m[2], l[2];         // M, and this lane's rows' share of the sum, of heads 2c and 2c + 1
   float acc[kG][2][4];      // [g][t]: dims 32 g + 4 r + 2 t (first two, 2^-22 n P') and the next one (last two, 2^-18 n P')
-  float sum[kG][4];         // sum of P'
+  float sum[kG][4];         // sum of 8 P', in the units of the two halves of acc
 
   __device__ __forceinline__ void start(const Kv4AttentionArgs& a, int b, int h) {
     const int lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
@@ -355,7 +364,7 @@ struct Attend {
         const uint32_t y1 = __byte_perm(x[2][g / 2], x[3][g / 2], g & 1 ? 0x7632 : 0x5410);
         mma_fp16(acc[g][0], y0 << 2 & 0x003C003Cu, y0 << 2 & 0x03C003C0u, y1 << 2 & 0x003C003Cu, y1 << 2 & 0x03C003C0u, b0, b1);
         mma_fp16(acc[g][1], y0 >> 6 & 0x003C003Cu, y0 >> 6 & 0x03C003C0u, y1 >> 6 & 0x003C003Cu, y1 >> 6 & 0x03C003C0u, b0, b1);
-        mma_fp16(sum[g], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0, b1);
+        mma_fp16(sum[g], 0x00200020u, 0x02000200u, 0x00200020u, 0x02000200u, b0, b1);
       }
     }
   }
@@ -363,9 +372,9 @@ struct Attend {
   // Weighted values of head 2c + j: dims 32 g + 4 r .. + 3.
   __device__ __forceinline__ float4 values(int g, int j) const {
     constexpr float kEven = 4194304.0f, kOdd = 262144.0f;      // 2^22, 2^18
-    const float e = 8.0f * sum[g][j];
-    return make_float4(fmaf(acc[g][0][j], kEven, -e), fmaf(acc[g][0][2 + j], kOdd, -e), fmaf(acc[g][1][j], kEven, -e),
-                       fmaf(acc[g][1][2 + j], kOdd, -e));
+    const float even = sum[g][j], odd = sum[g][2 + j];
+    return make_float4((acc[g][0][j] - even) * kEven, (acc[g][0][2 + j] - odd) * kOdd, (acc[g][1][j] - even) * kEven,
+                       (acc[g][1][2 + j] - odd) * kOdd);
   }
   // The piece: maxima, sums (after join_lanes), weighted values.
   __device__ __forceinline__ void leave(float* piece, int group) const {
@@ -424,6 +433,32 @@ __device__ __forceinline__ void append_row(const Kv4AttentionArgs& a, int b, int
   }
 }
 
+// Joins `n` pieces of one head into (m, l, four dims); `get(i, what)`: what = 0 the maximum, 1 the sum, and get4(i) the dims.  A
+// piece that saw no tile has a maximum of minus infinity and zeros; one whose scores were all NaN has the same maximum and
+// a sum of NaN, which stays one.
+template <int N, class Get, class Get4>
+__device__ __forceinline__ void join_pieces(int n, Get get, Get4 get4, float& m, float& l, float4& o) {
+  float mi[N], li[N];
+  float4 oi[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    mi[i] = i < n ? get(i, 0) : -INFINITY;
+    li[i] = i < n ? get(i, 1) : 0.0f;
+    oi[i] = i < n ? get4(i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  }
+  m = mi[0];
+#pragma unroll
+  for (int i = 1; i < N; ++i) m = fmaxf(m, mi[i]);
+  l = 0.0f;
+  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float f = mi[i] == -INFINITY ? 0.0f : exp2_of(mi[i] - m);
+    l += f * li[i];
+    o.x += f * oi[i].x; o.y += f * oi[i].y; o.z += f * oi[i].z; o.w += f * oi[i].w;
+  }
+}
+
 // A warp's copy of the tile that starts at row `slot` (of all heads) into a stage of its ring.
 template <int D>
 __device__ __forceinline__ void fetch_tile(const Kv4Cache& cache, size_t slot, uint32_t stage) {
@@ -452,6 +487,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   using L = Layout<D>;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int warp_sums[kWarps];
+  __shared__ FinalPiece final_of[kWarps];
   int* start = reinterpret_cast<int*>(smem + kWarps * kRing);      // [batch + 1]: first tile of a sequence
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hkv = a.cache.hkv;
   pdl_wait();
@@ -478,14 +514,14 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     __syncthreads();
   }
   const long long tiles = start[a.batch];
-  if (tiles == 0) return;
+  if (tiles == 0) return;      // every CTA
   const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
   const int first = first_tile(tiles, warps, w), end = first_tile(tiles, warps, w + 1);
-  if (first == end) return;
+  if (lane == 0) final_of[warp] = FinalPiece{first == end ? kNoTiles : kNoPiece, false, false, 0};
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
 
-  Cursor now;
-  {
+  Cursor now{0, 0, 0, 1};
+  if (first < end) {
     int lo = 0, hi = a.batch;      // the last sequence that starts at `first` or before and has tiles
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -551,69 +587,127 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     stage = stage == L::kStages - 1 ? 0 : stage + 1;
     if (last || i + 1 == end) {
       at.join_lanes();
-      const bool finished = last && whole;
-      if (finished) {
-        const int r = lane >> 2, c = lane & 3;
+      const int r = lane >> 2, c = lane & 3, bh = now.b * hkv + now.h;
+      if (last && whole) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int head = 2 * c + j;
           if (head >= a.group) continue;
           const float inv = 1.0f / at.l[j];
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + (((size_t)now.b * hkv + now.h) * a.group + head) * D + 4 * r;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(a.out) + ((size_t)bh * a.group + head) * D + 4 * r;
 #pragma unroll
           for (int g = 0; g < L::kGroups; ++g) {
             const float4 v = at.values(g, j);
             *reinterpret_cast<uint2*>(out + kGroup * g) =
                 make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
           }
-          if (kScores && r == 0)
-            ws.stats[((size_t)now.b * hkv + now.h) * kHeads + head] = make_float2(at.m[j], at.l[j]);
+          if (kScores && r == 0) ws.stats[(size_t)bh * kHeads + head] = make_float2(at.m[j], at.l[j]);
         }
-      } else {
-        at.leave(ws.pieces + ((size_t)w * 2 + (first_head ? 0 : 1)) * L::kPiece, a.group);
+      } else if (i + 1 < end) {      // the end of a head that other warps began
+        at.leave(ws.pieces + (size_t)w * 2 * L::kPiece, a.group);
+      } else {                       // stays in shared memory for the CTA's other warps
+        copy_wait<0>();
+        __syncwarp();
+        at.leave(reinterpret_cast<float*>(ring), a.group);
+        if (lane == 0) final_of[warp] = FinalPiece{bh, whole, last, first_head ? 0 : 1};
       }
       first_head = false;
       whole = true;
     }
     advance(now);
   }
-}
-
-__device__ __forceinline__ float block_reduce(float v, bool is_max, float* buf) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float y = __shfl_xor_sync(0xffffffffu, v, o);
-    v = is_max ? fmaxf(v, y) : v + y;
+  __syncthreads();
+  // Neighbouring warps that ended in the same head join their pieces: into the output where that is all of the head, else into
+  // the place of the first of them.
+  for (int w0 = 0; w0 < kWarps; ++w0) {
+    const FinalPiece lead = final_of[w0];
+    if (lead.head < 0) continue;
+    int w1 = w0 + 1;
+    bool last = lead.last;
+    while (w1 < kWarps && (final_of[w1].head == lead.head || final_of[w1].head == kNoTiles)) {
+      if (final_of[w1].head == lead.head) last = final_of[w1].last;
+      ++w1;
+    }
+    constexpr int kSide = D / 4, kSides = 32 * kWarps / kSide;      // threads a query head, four dims each
+    const int d = threadIdx.x % kSide;
+    for (int q = threadIdx.x / kSide; q < a.group; q += kSides) {
+      float m, l;
+      float4 o;
+      auto piece = [&](int k) { return reinterpret_cast<const float*>(smem + (w0 + k) * kRing); };
+      auto has = [&](int k) { return w0 + k < w1 && final_of[w0 + k].head == lead.head; };
+      join_pieces<kWarps>(
+          kWarps, [&](int k, int what) { return has(k) ? piece(k)[what * kHeads + q] : (what == 0 ? -INFINITY : 0.0f); },
+          [&](int k) {
+            return has(k) ? reinterpret_cast<const float4*>(piece(k))[(2 * kHeads + q * D) / 4 + d] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+          },
+          m, l, o);
+      if (lead.whole && last) {
+        const float inv = 1.0f / l;
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + ((size_t)lead.head * a.group + q) * D + 4 * d) =
+            make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+        if (kScores && d == 0) ws.stats[(size_t)lead.head * kHeads + q] = make_float2(m, l);
+      } else {
+        float* to = ws.pieces + ((size_t)(blockIdx.x * kWarps + w0) * 2 + lead.slot) * L::kPiece;
+        if (d == 0) {
+          to[q] = m;
+          to[kHeads + q] = l;
+        }
+        reinterpret_cast<float4*>(to)[(2 * kHeads + q * D) / 4 + d] = o;
+      }
+    }
+    w0 = w1 - 1;
   }
-  __syncthreads();
-  if (lane == 0) buf[warp] = v;
-  __syncthreads();
-  float r = buf[0];
-#pragma unroll
-  for (int i = 1; i < kJoinThreads / 32; ++i) r = is_max ? fmaxf(r, buf[i]) : r + buf[i];
-  return r;
 }
 
-// blockIdx.x: (sequence, kv head).  blockIdx.y < group: joins the pieces of that query head, where the head was cut.
-// blockIdx.y >= group: accumulates the weights of kJoinTiles tiles.
+// The pieces of a head whose tiles are [s0, s1) of the list.  Warps that ended in the same head of the same CTA left one piece, at
+// the first of them.
+template <int D>
+struct Pieces {
+  const Workspace& ws;
+  long long tiles;
+  int warps, s0, s1, wa, wb;
+  __device__ __forceinline__ Pieces(const Workspace& ws, long long tiles, int warps, int s0, int s1)
+      : ws(ws), tiles(tiles), warps(warps), s0(s0), s1(s1), wa(warp_of(tiles, warps, s0)), wb(warp_of(tiles, warps, s1 - 1)) {}
+  // Whether the first kernel has finished the head.
+  __device__ __forceinline__ bool finished() const {
+    return wa == wb || (wa / kWarps == wb / kWarps && first_tile(tiles, warps, wb + 1) == s1);
+  }
+  // The piece at warp w, or null if there is none.
+  __device__ __forceinline__ const float* at(int w) const {
+    const int f = first_tile(tiles, warps, w), e = first_tile(tiles, warps, w + 1);
+    if (f == e) return nullptr;
+    const bool joined = e <= s1 && f > max(s0, first_tile(tiles, warps, w / kWarps * kWarps));
+    return joined ? nullptr : ws.pieces + ((size_t)w * 2 + (f < s0 ? 1 : 0)) * Layout<D>::kPiece;
+  }
+};
+__device__ __forceinline__ void add_piece(float& m, float& l, float mi, float li) {
+  const float top = fmaxf(m, mi);
+  l = (m == -INFINITY ? 0.0f : exp2_of(m - top)) * l + (mi == -INFINITY ? 0.0f : exp2_of(mi - top)) * li;
+  m = top;
+}
+
+// blockIdx.x: (sequence, kv head).  blockIdx.y < outputs: joins the pieces of group / outputs query heads, where the head was
+// cut.  blockIdx.y >= outputs: accumulates the weights of every `chunks`-th kJoinTiles tiles.
 template <int D, bool kScores>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Kv4AttentionArgs a, int warps) {
-  using L = Layout<D>;
-  __shared__ float buf[kJoinThreads / 32];
-  __shared__ int sums[2][kJoinThreads / 32];
-  __shared__ float norms[2][kHeads], part[kJoinThreads / 32][kHeads];
-  __shared__ float4 halves[kJoinThreads / (D / 4)][D / 4];
-  const int bh = blockIdx.x, hkv = a.cache.hkv, b = bh / hkv, h = bh % hkv, tid = threadIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Kv4AttentionArgs a, int warps, int outputs,
+                                                            int chunks) {
+  constexpr int kJoinWarps = kJoinThreads / 32, kSide = D / 4, kLanes = 32 / kSide;      // kLanes pieces side by side in a warp
+  __shared__ int sums[2][kJoinWarps];
+  __shared__ float norms[2][kHeads];
+  __shared__ float part[kJoinWarps][2];
+  __shared__ float4 parts[kJoinWarps][kSide];
+  const int bh = blockIdx.x, hkv = a.cache.hkv, b = bh / hkv, h = bh % hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
+  pdl_launch_dependents();
   const int n = tiles_of(a, b);
   if (n == 0) {      // idle: the output row is zero
-    if ((int)blockIdx.y < a.group && tid < D / 8)
-      st_16(static_cast<__nv_bfloat16*>(a.out) + ((size_t)bh * a.group + blockIdx.y) * D + tid * 8, Vec16{0, 0, 0, 0});
+    if (blockIdx.y == 0)
+      for (int i = tid; i < a.group * D / 8; i += kJoinThreads)
+        st_16(static_cast<__nv_bfloat16*>(a.out) + (size_t)bh * a.group * D + i * 8, Vec16{0, 0, 0, 0});
     return;
   }
-  const int chunk = (int)blockIdx.y - a.group;
-  if (kScores && chunk >= 0 && chunk * kJoinTiles >= n) return;
+  const int chunk0 = (int)blockIdx.y - outputs;
+  if (kScores && chunk0 >= 0 && chunk0 * kJoinTiles >= n) return;
   int before = 0, all = 0;
   for (int i = tid; i < a.batch; i += kJoinThreads) {
     const int t = tiles_of(a, i);
@@ -625,128 +719,122 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     before += __shfl_xor_sync(0xffffffffu, before, o);
     all += __shfl_xor_sync(0xffffffffu, all, o);
   }
-  if ((tid & 31) == 0) {
-    sums[0][tid >> 5] = before;
-    sums[1][tid >> 5] = all;
+  if (lane == 0) {
+    sums[0][warp] = before;
+    sums[1][warp] = all;
   }
   __syncthreads();
   before = all = 0;
 #pragma unroll
-  for (int i = 0; i < kJoinThreads / 32; ++i) {
+  for (int i = 0; i < kJoinWarps; ++i) {
     before += sums[0][i];
     all += sums[1][i];
   }
-  const long long tiles = (long long)all * hkv;
-  const int s0 = before * hkv + h * n, s1 = s0 + n;
-  const int wa = warp_of(tiles, warps, s0), wb = warp_of(tiles, warps, s1 - 1);
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
-  // the piece of warp w, or null if it has no tiles
-  auto piece_of = [&](int w) -> const float* {
-    const int f = first_tile(tiles, warps, w);
-    if (f == first_tile(tiles, warps, w + 1)) return nullptr;
-    return ws.pieces + ((size_t)w * 2 + (f < s0 ? 1 : 0)) * L::kPiece;
-  };
-  if (chunk < 0) {
-    if (wa == wb) return;
-    const int q = blockIdx.y;
-    float m = -INFINITY;
-    for (int w = wa + tid; w <= wb; w += kJoinThreads) {
-      const float* p = piece_of(w);
-      if (p != nullptr) m = fmaxf(m, p[q]);
-    }
-    m = block_reduce(m, true, buf);
-    // D / 4 threads a piece, four dims each
-    constexpr int kSide = kJoinThreads / (D / 4);
-    const int side = tid / (D / 4), d = tid % (D / 4);
+  const int s0 = before * hkv + h * n;
+  const Pieces<D> pieces(ws, (long long)all * hkv, warps, s0, s0 + n);
+
+  if (chunk0 < 0) {
+    if (pieces.finished()) return;
+    // kJoinWarps / per warps a query head, each every `sides`-th group of pieces; four dims a thread
+    const int per = a.group / outputs, sides = kJoinWarps / per, q = blockIdx.y * per + warp / sides, side = warp % sides;
+    const int d = lane % kSide;
+    float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-#pragma unroll 4
-    for (int w = wa + side; w <= wb; w += kSide) {
-      const float* p = piece_of(w);
-      if (p == nullptr) continue;
-      const float f = exp2_of(p[q] - m);
-      const float4 v = *reinterpret_cast<const float4*>(p + 2 * kHeads + q * D + 4 * d);
-      o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
-      if (d == 0) sum += f * p[kHeads + q];
-    }
-    halves[side][d] = o;
-    sum = block_reduce(sum, false, buf);      // synchronises
-    if (side == 0) {
-      for (int i = 1; i < kSide; ++i) {
-        o.x += halves[i][d].x; o.y += halves[i][d].y; o.z += halves[i][d].z; o.w += halves[i][d].w;
+    if (warp < per * sides) {
+      for (int w = pieces.wa + lane; w <= pieces.wb; w += 32) {      // the maximum first, so that every piece is scaled once
+        const float* p = pieces.at(w);
+        if (p != nullptr) m = fmaxf(m, p[q]);
       }
-      const float inv = 1.0f / sum;
+#pragma unroll
+      for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
+#pragma unroll 4
+      for (int w = pieces.wa + side * kLanes + lane / kSide; w <= pieces.wb; w += sides * kLanes) {
+        const float* p = pieces.at(w);
+        if (p == nullptr) continue;
+        const float f = p[q] == -INFINITY ? 0.0f : exp2_of(p[q] - m);
+        const float4 v = *reinterpret_cast<const float4*>(p + 2 * kHeads + q * D + 4 * d);
+        l += f * p[kHeads + q];
+        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+      }
+      if (kLanes == 2) {
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        o.x += __shfl_xor_sync(0xffffffffu, o.x, 16); o.y += __shfl_xor_sync(0xffffffffu, o.y, 16);
+        o.z += __shfl_xor_sync(0xffffffffu, o.z, 16); o.w += __shfl_xor_sync(0xffffffffu, o.w, 16);
+      }
+      if (lane < kSide) parts[warp][d] = o;
+      if (lane == 0) part[warp][0] = l;
+    }
+    __syncthreads();
+    if (warp < per * sides && side == 0 && lane < kSide) {
+      for (int i = 1; i < sides; ++i) {
+        const float4 v = parts[warp + i][d];
+        o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
+        l += part[warp + i][0];
+      }
+      const float inv = 1.0f / l;
       *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + ((size_t)bh * a.group + q) * D + 4 * d) =
           make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
     }
     return;
   }
   if constexpr (kScores) {
-    // what this thread accumulates comes in while the heads' maxima and sums are found
+    // a chunk comes in while the heads' maxima and sums are found, and the next one while this one is worked on
     constexpr int kMine = kJoinTiles * kTile / kJoinThreads;
-    const int q = tid % kHeads, pitch = padded_group(a.group), len = length_of(a, b), i0 = chunk * kJoinTiles * kTile + tid;
+    const int pitch = padded_group(a.group), len = length_of(a, b);
     const float* scores = ws.scores + (size_t)s0 * kTile * pitch;
+    float* weights = a.cache.weights + (size_t)bh * a.cache.slots;
     float2 x[kMine][kHeads / 2];
     float weight[kMine];
+    auto fetch = [&](int chunk) {
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int i = i0 + k * kJoinThreads;
-      if (i > len) continue;
-      weight[k] = a.cache.weights[(size_t)bh * a.cache.slots + i];
+      for (int k = 0; k < kMine; ++k) {
+        const int i = chunk * kJoinTiles * kTile + k * kJoinThreads + tid;
+        if (i > len) continue;
+        weight[k] = weights[i];
 #pragma unroll
-      for (int j = 0; j < kHeads / 2; ++j)
-        if (2 * j < a.group) x[k][j] = *reinterpret_cast<const float2*>(scores + (size_t)i * pitch + 2 * j);
-    }
-    if (wa == wb) {
-      if (tid < kHeads && q < a.group) {
-        const float2 s = ws.stats[(size_t)bh * kHeads + q];
-        norms[0][q] = s.x;
-        norms[1][q] = 1.0f / s.y;
+        for (int j = 0; j < kHeads / 2; ++j)
+          if (2 * j < a.group) x[k][j] = *reinterpret_cast<const float2*>(scores + (size_t)i * pitch + 2 * j);
       }
-    } else {
-      float m = -INFINITY, sum = 0.0f;
-      if (q < a.group)
-        for (int w = wa + tid / kHeads; w <= wb; w += kJoinThreads / kHeads) {
-          const float* p = piece_of(w);
-          if (p != nullptr) m = fmaxf(m, p[q]);
+    };
+    fetch(chunk0);
+    if (warp < a.group) {      // a warp a query head
+      float m = -INFINITY, l = 0.0f;
+      if (pieces.finished()) {
+        const float2 s = ws.stats[(size_t)bh * kHeads + warp];
+        m = s.x;
+        l = s.y;
+      } else {
+        for (int w = pieces.wa + lane; w <= pieces.wb; w += 32) {
+          const float* p = pieces.at(w);
+          if (p != nullptr) add_piece(m, l, p[warp], p[kHeads + warp]);
         }
 #pragma unroll
-      for (int o = kHeads; o < 32; o <<= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      if ((tid & 31) < kHeads) part[tid >> 5][q] = m;
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < kJoinThreads / 32; ++i) m = fmaxf(m, part[i][q]);
-      __syncthreads();
-      if (q < a.group)
-        for (int w = wa + tid / kHeads; w <= wb; w += kJoinThreads / kHeads) {
-          const float* p = piece_of(w);
-          if (p != nullptr) sum += exp2_of(p[q] - m) * p[kHeads + q];
+        for (int k = 16; k > 0; k >>= 1) {
+          const float mi = __shfl_xor_sync(0xffffffffu, m, k), li = __shfl_xor_sync(0xffffffffu, l, k);
+          add_piece(m, l, mi, li);
         }
-#pragma unroll
-      for (int o = kHeads; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if ((tid & 31) < kHeads) part[tid >> 5][q] = sum;
-      __syncthreads();
-      if (tid < kHeads) {
-        sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < kJoinThreads / 32; ++i) sum += part[i][q];
-        norms[0][q] = m;
-        norms[1][q] = 1.0f / sum;
+      }
+      if (lane == 0) {
+        norms[0][warp] = m;
+        norms[1][warp] = 1.0f / l;
       }
     }
     __syncthreads();
-    float* weights = a.cache.weights + (size_t)bh * a.cache.slots;
+    for (int chunk = chunk0; chunk * kJoinTiles < n; chunk += chunks) {
+      if (chunk != chunk0) fetch(chunk);
 #pragma unroll
-    for (int k = 0; k < kMine; ++k) {
-      const int i = i0 + k * kJoinThreads;
-      if (i > len) continue;
-      float p = 0.0f;
+      for (int k = 0; k < kMine; ++k) {
+        const int i = chunk * kJoinTiles * kTile + k * kJoinThreads + tid;
+        if (i > len) continue;
+        float p = 0.0f;
 #pragma unroll
-      for (int j = 0; j < kHeads / 2; ++j) {
-        if (2 * j < a.group) p += exp2_of(x[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
-        if (2 * j + 1 < a.group) p += exp2_of(x[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
+        for (int j = 0; j < kHeads / 2; ++j) {
+          if (2 * j < a.group) p += exp2_of(x[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
+          if (2 * j + 1 < a.group) p += exp2_of(x[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
+        }
+        weights[i] = i == len ? p : weight[k] + p;
       }
-      weights[i] = i == len ? p : weight[k] + p;
     }
   }
 }
@@ -777,32 +865,6 @@ __device__ __forceinline__ float4 load_remote_4(uint32_t addr) {
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
-// Joins `n` pieces of one head into (m, l, four dims); `get(i, what)`: what = 0 the maximum, 1 the sum, and get4(i) the dims.  A
-// piece that saw no tile has a maximum of minus infinity and zeros; one whose scores were all NaN has the same maximum and
-// a sum of NaN, which stays one.
-template <int N, class Get, class Get4>
-__device__ __forceinline__ void join_pieces(int n, Get get, Get4 get4, float& m, float& l, float4& o) {
-  float mi[N], li[N];
-  float4 oi[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    mi[i] = i < n ? get(i, 0) : -INFINITY;
-    li[i] = i < n ? get(i, 1) : 0.0f;
-    oi[i] = i < n ? get4(i) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  }
-  m = mi[0];
-#pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, mi[i]);
-  l = 0.0f;
-  o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float f = mi[i] == -INFINITY ? 0.0f : exp2_of(mi[i] - m);
-    l += f * li[i];
-    o.x += f * oi[i].x; o.y += f * oi[i].y; o.z += f * oi[i].z; o.w += f * oi[i].w;
-  }
-}
 
 template <int D, bool kScores>
 __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const __grid_constant__ Kv4AttentionArgs a, int ctas,
@@ -975,9 +1037,12 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
   const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
   if (int e = launch_kernel(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
-  const int chunks = kScores ? (tiles + kJoinTiles - 1) / kJoinTiles : 0;
-  return launch_kernel(join_kernel<D, kScores>, dim3(a.batch * a.cache.hkv, a.group + chunks), kJoinThreads, 0, 1, stream, a,
-                       ctas * kWarps);
+  // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; the weights' CTAs fill the GPU once.
+  const int heads = a.batch * a.cache.hkv, resident = 3 * a.num_sms;
+  const int outputs = heads * a.group <= 2 * resident ? a.group : 1;
+  const int chunks = kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, resident / heads)) : 0;
+  return launch_kernel(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
+                       chunks);
 }
 
 }  // namespace
