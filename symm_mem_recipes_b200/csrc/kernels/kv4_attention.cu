@@ -75,11 +75,17 @@ __device__ __forceinline__ int tiles_of(const Kv4AttentionArgs& a, int b) {
   const int n = length_of(a, b);
   return n >= 0 && n < a.cache.max_seq ? n / kTile + 1 : 0;
 }
-// First tile of a warp, and the warp that has a tile.
-__device__ __forceinline__ int first_tile(long long tiles, int warps, int w) { return (int)(tiles * w / warps); }
-__device__ __forceinline__ int warp_of(long long tiles, int warps, int tile) {
-  return (int)(((long long)(tile + 1) * warps - 1) / tiles);
-}
+// The list's tiles among the warps: the first `more` of them have one tile more than the others.  (One 32-bit division; with
+// tiles * w / warps in 64 bits the second kernel spent 20 us on divisions.)
+struct Shares {
+  int tiles, each, more;
+  __device__ __forceinline__ Shares(int tiles, int warps) : tiles(tiles), each(tiles / warps), more(tiles - each * warps) {}
+  __device__ __forceinline__ int first(int w) const { return w * each + min(w, more); }
+  __device__ __forceinline__ int warp_of(int tile) const {
+    const int of_more = more * (each + 1);
+    return tile < of_more ? tile / (each + 1) : more + (tile - of_more) / each;      // each > 0 where a tile is behind those
+  }
+};
 
 __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -513,10 +519,11 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     if (threadIdx.x == 32 * kWarps - 1) start[a.batch] = before;
     __syncthreads();
   }
-  const long long tiles = start[a.batch];
+  const int tiles = start[a.batch];
   if (tiles == 0) return;      // every CTA
   const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
-  const int first = first_tile(tiles, warps, w), end = first_tile(tiles, warps, w + 1);
+  const Shares shares(tiles, warps);
+  const int first = shares.first(w), end = shares.first(w + 1);
   if (lane == 0) final_of[warp] = FinalPiece{first == end ? kNoTiles : kNoPiece, false, false, 0};
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
 
@@ -664,19 +671,19 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
 template <int D>
 struct Pieces {
   const Workspace& ws;
-  long long tiles;
-  int warps, s0, s1, wa, wb;
-  __device__ __forceinline__ Pieces(const Workspace& ws, long long tiles, int warps, int s0, int s1)
-      : ws(ws), tiles(tiles), warps(warps), s0(s0), s1(s1), wa(warp_of(tiles, warps, s0)), wb(warp_of(tiles, warps, s1 - 1)) {}
+  Shares shares;
+  int s0, s1, wa, wb;
+  __device__ __forceinline__ Pieces(const Workspace& ws, int tiles, int warps, int s0, int s1)
+      : ws(ws), shares(tiles, warps), s0(s0), s1(s1), wa(shares.warp_of(s0)), wb(shares.warp_of(s1 - 1)) {}
   // Whether the first kernel has finished the head.
   __device__ __forceinline__ bool finished() const {
-    return wa == wb || (wa / kWarps == wb / kWarps && first_tile(tiles, warps, wb + 1) == s1);
+    return wa == wb || (wa / kWarps == wb / kWarps && shares.first(wb + 1) == s1);
   }
   // The piece at warp w, or null if there is none.
   __device__ __forceinline__ const float* at(int w) const {
-    const int f = first_tile(tiles, warps, w), e = first_tile(tiles, warps, w + 1);
+    const int f = shares.first(w), e = shares.first(w + 1);
     if (f == e) return nullptr;
-    const bool joined = e <= s1 && f > max(s0, first_tile(tiles, warps, w / kWarps * kWarps));
+    const bool joined = e <= s1 && f > max(s0, shares.first(w / kWarps * kWarps));
     return joined ? nullptr : ws.pieces + ((size_t)w * 2 + (f < s0 ? 1 : 0)) * Layout<D>::kPiece;
   }
 };
@@ -732,7 +739,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   }
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
   const int s0 = before * hkv + h * n;
-  const Pieces<D> pieces(ws, (long long)all * hkv, warps, s0, s0 + n);
+  const Pieces<D> pieces(ws, all * hkv, warps, s0, s0 + n);
 
   if (chunk0 < 0) {
     if (pieces.finished()) return;
