@@ -41,7 +41,7 @@ constexpr int kWarps = 4;                 // of an attention CTA
 constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
 constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
 constexpr int kJoinThreads = 256;
-constexpr int kJoinTiles = 16;            // tiles whose weights a CTA of the second kernel accumulates at a time
+constexpr int kJoinTiles = 8;             // tiles whose weights a CTA of the second kernel accumulates at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -666,25 +666,26 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   }
 }
 
-// The pieces of a head whose tiles are [s0, s1) of the list.  Warps that ended in the same head of the same CTA left one piece, at
-// the first of them.
+// The pieces of a head whose tiles are [s0, s1) of the list: one of every CTA that has some, at the first of its warps that does
+// (warps that ended in the head joined theirs), and one more of the last warp, where that went on to another head and is not
+// the first itself.
 template <int D>
 struct Pieces {
   const Workspace& ws;
   Shares shares;
-  int s0, s1, wa, wb;
+  int s0, wa, wb, ctas, count;
+  bool finished;      // by the first kernel
   __device__ __forceinline__ Pieces(const Workspace& ws, int tiles, int warps, int s0, int s1)
-      : ws(ws), shares(tiles, warps), s0(s0), s1(s1), wa(shares.warp_of(s0)), wb(shares.warp_of(s1 - 1)) {}
-  // Whether the first kernel has finished the head.
-  __device__ __forceinline__ bool finished() const {
-    return wa == wb || (wa / kWarps == wb / kWarps && shares.first(wb + 1) == s1);
+      : ws(ws), shares(tiles, warps), s0(s0), wa(shares.warp_of(s0)), wb(shares.warp_of(s1 - 1)) {
+    const int ca = wa / kWarps, cb = wb / kWarps;
+    const bool ends = shares.first(wb + 1) == s1;
+    ctas = cb - ca + 1;
+    count = ctas + (!ends && wb != max(wa, cb * kWarps) ? 1 : 0);
+    finished = wa == wb || (ca == cb && ends);
   }
-  // The piece at warp w, or null if there is none.
-  __device__ __forceinline__ const float* at(int w) const {
-    const int f = shares.first(w), e = shares.first(w + 1);
-    if (f == e) return nullptr;
-    const bool joined = e <= s1 && f > max(s0, shares.first(w / kWarps * kWarps));
-    return joined ? nullptr : ws.pieces + ((size_t)w * 2 + (f < s0 ? 1 : 0)) * Layout<D>::kPiece;
+  __device__ __forceinline__ const float* at(int k) const {
+    const int w = k == 0 ? wa : k < ctas ? (wa / kWarps + k) * kWarps : wb;
+    return ws.pieces + ((size_t)w * 2 + (shares.first(w) < s0 ? 1 : 0)) * Layout<D>::kPiece;
   }
 };
 __device__ __forceinline__ void add_piece(float& m, float& l, float mi, float li) {
@@ -742,23 +743,19 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const Pieces<D> pieces(ws, all * hkv, warps, s0, s0 + n);
 
   if (chunk0 < 0) {
-    if (pieces.finished()) return;
+    if (pieces.finished) return;
     // kJoinWarps / per warps a query head, each every `sides`-th group of pieces; four dims a thread
     const int per = a.group / outputs, sides = kJoinWarps / per, q = blockIdx.y * per + warp / sides, side = warp % sides;
     const int d = lane % kSide;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (warp < per * sides) {
-      for (int w = pieces.wa + lane; w <= pieces.wb; w += 32) {      // the maximum first, so that every piece is scaled once
-        const float* p = pieces.at(w);
-        if (p != nullptr) m = fmaxf(m, p[q]);
-      }
+      for (int k = lane; k < pieces.count; k += 32) m = fmaxf(m, pieces.at(k)[q]);      // first, so that every piece is scaled once
 #pragma unroll
       for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
 #pragma unroll 4
-      for (int w = pieces.wa + side * kLanes + lane / kSide; w <= pieces.wb; w += sides * kLanes) {
-        const float* p = pieces.at(w);
-        if (p == nullptr) continue;
+      for (int k = side * kLanes + lane / kSide; k < pieces.count; k += sides * kLanes) {
+        const float* p = pieces.at(k);
         const float f = p[q] == -INFINITY ? 0.0f : exp2_of(p[q] - m);
         const float4 v = *reinterpret_cast<const float4*>(p + 2 * kHeads + q * D + 4 * d);
         l += f * p[kHeads + q];
@@ -786,36 +783,36 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     return;
   }
   if constexpr (kScores) {
-    // a chunk comes in while the heads' maxima and sums are found, and the next one while this one is worked on
+    // the first slots' scores come in while the heads' maxima and sums are found, the next ones while these are worked on
     constexpr int kMine = kJoinTiles * kTile / kJoinThreads;
     const int pitch = padded_group(a.group), len = length_of(a, b);
     const float* scores = ws.scores + (size_t)s0 * kTile * pitch;
     float* weights = a.cache.weights + (size_t)bh * a.cache.slots;
-    float2 x[kMine][kHeads / 2];
-    float weight[kMine];
-    auto fetch = [&](int chunk) {
+    struct Mine {
+      float2 s[kMine][kHeads / 2];
+      float weight[kMine];
+    };
+    auto fetch = [&](int chunk, Mine& x) {
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
         const int i = chunk * kJoinTiles * kTile + k * kJoinThreads + tid;
         if (i > len) continue;
-        weight[k] = weights[i];
+        x.weight[k] = weights[i];
 #pragma unroll
         for (int j = 0; j < kHeads / 2; ++j)
-          if (2 * j < a.group) x[k][j] = *reinterpret_cast<const float2*>(scores + (size_t)i * pitch + 2 * j);
+          if (2 * j < a.group) x.s[k][j] = *reinterpret_cast<const float2*>(scores + (size_t)i * pitch + 2 * j);
       }
     };
-    fetch(chunk0);
+    Mine x;
+    fetch(chunk0, x);
     if (warp < a.group) {      // a warp a query head
       float m = -INFINITY, l = 0.0f;
-      if (pieces.finished()) {
+      if (pieces.finished) {
         const float2 s = ws.stats[(size_t)bh * kHeads + warp];
         m = s.x;
         l = s.y;
       } else {
-        for (int w = pieces.wa + lane; w <= pieces.wb; w += 32) {
-          const float* p = pieces.at(w);
-          if (p != nullptr) add_piece(m, l, p[warp], p[kHeads + warp]);
-        }
+        for (int k = lane; k < pieces.count; k += 32) add_piece(m, l, pieces.at(k)[warp], pieces.at(k)[kHeads + warp]);
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) {
           const float mi = __shfl_xor_sync(0xffffffffu, m, k), li = __shfl_xor_sync(0xffffffffu, l, k);
@@ -829,7 +826,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     }
     __syncthreads();
     for (int chunk = chunk0; chunk * kJoinTiles < n; chunk += chunks) {
-      if (chunk != chunk0) fetch(chunk);
+      Mine ahead;
+      fetch(chunk + chunks, ahead);
 #pragma unroll
       for (int k = 0; k < kMine; ++k) {
         const int i = chunk * kJoinTiles * kTile + k * kJoinThreads + tid;
@@ -837,11 +835,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         float p = 0.0f;
 #pragma unroll
         for (int j = 0; j < kHeads / 2; ++j) {
-          if (2 * j < a.group) p += exp2_of(x[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
-          if (2 * j + 1 < a.group) p += exp2_of(x[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
+          if (2 * j < a.group) p += exp2_of(x.s[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
+          if (2 * j + 1 < a.group) p += exp2_of(x.s[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
         }
-        weights[i] = i == len ? p : weight[k] + p;
+        weights[i] = i == len ? p : x.weight[k] + p;
       }
+      x = ahead;
     }
   }
 }
@@ -1045,7 +1044,7 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
   if (int e = launch_kernel(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
   // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; the weights' CTAs fill the GPU once.
-  const int heads = a.batch * a.cache.hkv, resident = 3 * a.num_sms;
+  const int heads = a.batch * a.cache.hkv, resident = 4 * a.num_sms;
   const int outputs = heads * a.group <= 2 * resident ? a.group : 1;
   const int chunks = kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, resident / heads)) : 0;
   return launch_kernel(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
