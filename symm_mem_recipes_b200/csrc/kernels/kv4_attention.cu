@@ -87,8 +87,13 @@ struct Shares {
   }
 };
 
-__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+// kOnce: the lines are the first to leave L2, where others are wanted again.
+template <bool kOnce>
+__device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, uint64_t policy) {
+  if constexpr (kOnce)
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+  else
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -465,26 +470,29 @@ __device__ __forceinline__ void join_pieces(int n, Get get, Get4 get4, float& m,
   }
 }
 
-// A warp's copy of the tile that starts at row `slot` (of all heads) into a stage of its ring.
-template <int D>
+// A warp's copy of the tile that starts at row `slot` (of all heads) into a stage of its ring.  Where scores are kept for the second
+// kernel the cache's lines make room for them in L2 (kOnce).
+template <int D, bool kOnce>
 __device__ __forceinline__ void fetch_tile(const Kv4Cache& cache, size_t slot, uint32_t stage) {
   using L = Layout<D>;
   const int lane = threadIdx.x & 31;
+  uint64_t policy = 0;
+  if constexpr (kOnce) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
   const uint32_t dst = stage + lane * 16;
   const uint8_t* kc = cache.k_codes + slot * (D / 2) + lane * 16;
   const uint8_t* vc = cache.v_codes + slot * (D / 2) + lane * 16;
 #pragma unroll
   for (int i = 0; i < L::kCodes / 512; ++i) {
-    copy_async_16(dst + i * 512, kc + i * 512);
-    copy_async_16(dst + L::kCodes + i * 512, vc + i * 512);
+    copy_async_16<kOnce>(dst + i * 512, kc + i * 512, policy);
+    copy_async_16<kOnce>(dst + L::kCodes + i * 512, vc + i * 512, policy);
   }
   const uint8_t* ks = static_cast<const uint8_t*>(cache.k_scales) + slot * (2 * L::kGroups);
   const uint8_t* vs = static_cast<const uint8_t*>(cache.v_scales) + slot * (2 * L::kGroups);
   if constexpr (D == 128) {
-    copy_async_16(dst + 2 * L::kCodes, ks + lane * 16);
-    copy_async_16(dst + 2 * L::kCodes + L::kScales, vs + lane * 16);
+    copy_async_16<kOnce>(dst + 2 * L::kCodes, ks + lane * 16, policy);
+    copy_async_16<kOnce>(dst + 2 * L::kCodes + L::kScales, vs + lane * 16, policy);
   } else {      // 256 bytes of either, half a warp each
-    copy_async_16(dst + 2 * L::kCodes, lane < 16 ? ks + lane * 16 : vs + (lane - 16) * 16);
+    copy_async_16<kOnce>(dst + 2 * L::kCodes, lane < 16 ? ks + lane * 16 : vs + (lane - 16) * 16, policy);
   }
 }
 
@@ -492,54 +500,69 @@ template <int D, bool kScores>
 __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_constant__ Kv4AttentionArgs a) {
   using L = Layout<D>;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int warp_sums[kWarps];
   __shared__ FinalPiece final_of[kWarps];
   int* start = reinterpret_cast<int*>(smem + kWarps * kRing);      // [batch + 1]: first tile of a sequence
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hkv = a.cache.hkv;
+  if (lane == 0) final_of[warp] = FinalPiece{kNoTiles, false, false, 0};
   pdl_wait();
   pdl_launch_dependents();
-  {
-    const int per = (a.batch + 32 * kWarps - 1) / (32 * kWarps), b0 = threadIdx.x * per;
-    int sum = 0;
-    for (int i = 0; i < per; ++i) sum += b0 + i < a.batch ? tiles_of(a, b0 + i) * hkv : 0;
-    int x = sum;
+  // Every warp finds its first tile by itself, so that the copies start without a barrier; the first one leaves the sequences' first
+  // tiles for later.
+  const int per = (a.batch + 31) / 32, b0 = lane * per;
+  int mine = 0;
+  for (int i = 0; i < per; ++i) mine += b0 + i < a.batch ? tiles_of(a, b0 + i) * hkv : 0;
+  int before = mine;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  const int tiles = __shfl_sync(0xffffffffu, before, 31);
+  if (tiles == 0) return;      // every CTA
+  before -= mine;
+  const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
+  const Shares shares(tiles, warps);
+  const int first = shares.first(w), end = shares.first(w + 1);
+  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
+  Cursor now{0, 0, 0, 1};
+  if (first < end) {
+    int left = first - before;      // of the sequence that `first` is in, in the lane that has it
+    const bool has = left >= 0 && left < mine;
+    if (has) {
+      now.b = b0;
+      while (left >= (now.n = tiles_of(a, now.b)) * hkv) {
+        left -= now.n * hkv;
+        ++now.b;
+      }
+      now.h = left / now.n;
+      now.t = left - now.h * now.n;
     }
-    if (lane == 31) warp_sums[warp] = x;
-    __syncthreads();
-    int before = x - sum;
-    for (int i = 0; i < warp; ++i) before += warp_sums[i];
+    const int from = __ffs(__ballot_sync(0xffffffffu, has)) - 1;
+    now.b = __shfl_sync(0xffffffffu, now.b, from);
+    now.h = __shfl_sync(0xffffffffu, now.h, from);
+    now.t = __shfl_sync(0xffffffffu, now.t, from);
+    now.n = __shfl_sync(0xffffffffu, now.n, from);
+  }
+  uint8_t* ring = smem + warp * kRing;
+  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
+  auto fetch = [&](const Cursor& at, int stage) {
+    fetch_tile<D, kScores>(a.cache, ((size_t)at.b * hkv + at.h) * a.cache.slots + (size_t)at.t * kTile, ring_addr + stage * L::kBytes);
+  };
+  int to_fetch = first;
+  if (to_fetch < end) {
+    fetch(now, 0);
+    ++to_fetch;
+    if (lane == 0) final_of[warp].head = kNoPiece;
+  }
+  copy_commit();
+  if (warp == 0) {
     for (int i = 0; i < per && b0 + i < a.batch; ++i) {
       start[b0 + i] = before;
       before += tiles_of(a, b0 + i) * hkv;
     }
-    if (threadIdx.x == 32 * kWarps - 1) start[a.batch] = before;
-    __syncthreads();
+    if (lane == 31) start[a.batch] = tiles;
   }
-  const int tiles = start[a.batch];
-  if (tiles == 0) return;      // every CTA
-  const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
-  const Shares shares(tiles, warps);
-  const int first = shares.first(w), end = shares.first(w + 1);
-  if (lane == 0) final_of[warp] = FinalPiece{first == end ? kNoTiles : kNoPiece, false, false, 0};
-  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
-
-  Cursor now{0, 0, 0, 1};
-  if (first < end) {
-    int lo = 0, hi = a.batch;      // the last sequence that starts at `first` or before and has tiles
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (start[mid] <= first) lo = mid;
-      else hi = mid;
-    }
-    now.b = lo;
-    now.n = (start[lo + 1] - start[lo]) / hkv;
-    now.h = (first - start[lo]) / now.n;
-    now.t = first - start[lo] - now.h * now.n;
-  }
+  __syncthreads();
   auto advance = [&](Cursor& at) {
     if (++at.t < at.n) return;
     at.t = 0;
@@ -550,18 +573,12 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     } while (at.b < a.batch && start[at.b + 1] == start[at.b]);
     if (at.b < a.batch) at.n = (start[at.b + 1] - start[at.b]) / hkv;
   };
-  uint8_t* ring = smem + warp * kRing;
-  const uint32_t ring_addr = (uint32_t)__cvta_generic_to_shared(ring);
-  auto fetch = [&](const Cursor& at, int stage) {
-    fetch_tile<D>(a.cache, ((size_t)at.b * hkv + at.h) * a.cache.slots + (size_t)at.t * kTile, ring_addr + stage * L::kBytes);
-  };
   Cursor ahead = now;
-  int to_fetch = first;
 #pragma unroll
-  for (int i = 0; i < L::kStages - 1; ++i) {
+  for (int i = 1; i < L::kStages - 1; ++i) {
     if (to_fetch < end) {
-      fetch(ahead, i);
       advance(ahead);
+      fetch(ahead, i);
       ++to_fetch;
     }
     copy_commit();
@@ -576,8 +593,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     copy_wait<L::kStages - 2>();
     __syncwarp();      // the tile is there for every lane, and every lane is done with the stage that is filled next
     if (to_fetch < end) {
-      fetch(ahead, stage == 0 ? L::kStages - 1 : stage - 1);
       advance(ahead);
+      fetch(ahead, stage == 0 ? L::kStages - 1 : stage - 1);
       ++to_fetch;
     }
     copy_commit();
@@ -705,10 +722,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   __shared__ float part[kJoinWarps][2];
   __shared__ float4 parts[kJoinWarps][kSide];
   const int bh = blockIdx.x, hkv = a.cache.hkv, b = bh / hkv, h = bh % hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_wait();
-  pdl_launch_dependents();
+  // The lengths are no output of the first kernel: it has waited for what wrote them before it let this one start.
   const int n = tiles_of(a, b);
   if (n == 0) {      // idle: the output row is zero
+    pdl_wait();
     if (blockIdx.y == 0)
       for (int i = tid; i < a.group * D / 8; i += kJoinThreads)
         st_16(static_cast<__nv_bfloat16*>(a.out) + (size_t)bh * a.group * D + i * 8, Vec16{0, 0, 0, 0});
@@ -740,8 +757,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   }
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
   const int s0 = before * hkv + h * n;
+  pdl_launch_dependents();
   const Pieces<D> pieces(ws, all * hkv, warps, s0, s0 + n);
 
+  pdl_wait();
   if (chunk0 < 0) {
     if (pieces.finished) return;
     // kJoinWarps / per warps a query head, each every `sides`-th group of pieces; four dims a thread
@@ -898,7 +917,7 @@ __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const _
 #pragma unroll
   for (int i = 0; i < kHeadStages; ++i) {
     const int t = first + i * step;
-    if (t < n) fetch_tile<D>(a.cache, base + (size_t)t * kTile, ring_addr + i * L::kBytes);
+    if (t < n) fetch_tile<D, false>(a.cache, base + (size_t)t * kTile, ring_addr + i * L::kBytes);
     copy_commit();
   }
   Attend<D, kScores> at;
@@ -916,7 +935,7 @@ __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const _
     at.tile(stage, valid, scores + i * kTile * pitch, a.group, pitch);
     __syncwarp();
     const int next = t + kHeadStages * step;
-    if (next < n) fetch_tile<D>(a.cache, base + (size_t)next * kTile, ring_addr + (i % kHeadStages) * L::kBytes);
+    if (next < n) fetch_tile<D, false>(a.cache, base + (size_t)next * kTile, ring_addr + (i % kHeadStages) * L::kBytes);
     copy_commit();
   }
   copy_wait<0>();
