@@ -15,7 +15,9 @@ projections use the fused GEMV + all-reduce.  It continues from KV caches that
 the prefill fills when given `kv_cache=(k_cache, v_cache)`.  `decode_static` is the same step
 with shapes and launches independent of the position, and `DecodeGraph`
 captures it (through any number of layers) in one CUDA graph that is replayed
-per token.
+per token.  With a 4-bit cache (`ops.Kv4Cache`) the step is `decode_kv4`, and
+`Kv4DecodeGraph` its graph: sequences have lengths and positions of their own,
+and may be cut to the slots that attention has weighed most.
 
 Prefill without sequence parallelism (`forward_tp`), activations replicated:
 local GEMMs for the column-parallel projections, `matmul_all_reduce` for the
@@ -213,6 +215,13 @@ class LlamaTPDecoderLayer:
                                                is_causal=True, enable_gqa=True)
         return o.transpose(1, 2).reshape(batch * seq, hq * D).contiguous()
 
+    def _prompt_buffers(self, cache: "ops.Kv4Cache", batch: int, seq: int):
+        """Where a prompt's keys and values are in 16 bits on their way into a 4-bit cache."""
+        if cache.batch != batch or cache.max_seq < seq or cache.n_kv_heads != self.hkv or cache.head_dim != self.cfg.head_dim:
+            raise ValueError("kv_cache: a Kv4Cache of this batch, kv heads per rank and head_dim, with max_seq >= seq")
+        k = torch.empty(batch, seq, self.hkv, self.cfg.head_dim, dtype=torch.bfloat16, device=self.device)
+        return k, torch.empty_like(k)
+
     @staticmethod
     def _mlp_act_torch(gu: torch.Tensor, ffn_local: int) -> torch.Tensor:
         gate, up = gu.split(ffn_local, dim=-1)
@@ -237,10 +246,16 @@ class LlamaTPDecoderLayer:
     def forward(self, x_shard: torch.Tensor, batch: int, seq: int, barrier_between_phases: bool = False,
                 kv_cache=None) -> torch.Tensor:
         """x_shard [batch*seq/WS, H] (this rank's tokens) -> same shape.  `kv_cache = (k_cache,
-        v_cache)` receives this rank's keys and values of the prompt, for `decode` to continue from."""
+        v_cache)` receives this rank's keys and values of the prompt, for `decode` to continue from; an
+        `ops.Kv4Cache` receives them in four bits, for `decode_kv4` (the prompt's own attention sees them in 16)."""
         cfg = self.cfg
         rows = x_shard.shape[0]
         assert rows * self.ws == batch * seq
+        if isinstance(kv_cache, ops.Kv4Cache):
+            k, v = self._prompt_buffers(kv_cache, batch, seq)
+            y = self.forward(x_shard, batch, seq, barrier_between_phases, kv_cache=(k, v))
+            ops.kv4_append_(k, v, kv_cache)
+            return y
         if not barrier_between_phases and self.phase_marks is None:
             y = self._prefill_local(x_shard, batch, seq, kv_cache)
             if y is not None:
@@ -292,6 +307,11 @@ class LlamaTPDecoderLayer:
         full [batch*seq, H] output, identical on every rank."""
         cfg = self.cfg
         assert x.shape[0] == batch * seq
+        if isinstance(kv_cache, ops.Kv4Cache):
+            k, v = self._prompt_buffers(kv_cache, batch, seq)
+            y = self.forward_tp(x, batch, seq, kv_cache=(k, v))
+            ops.kv4_append_(k, v, kv_cache)
+            return y
         y = self._prefill_local(x, batch, seq, kv_cache)
         if y is not None:
             return y
@@ -462,6 +482,24 @@ class LlamaTPDecoderLayer:
         return self._decode_mlp(x, o_proj, fused, glue)
 
 
+    def decode_kv4(self, x: torch.Tensor, cache: "ops.Kv4Cache", lengths: torch.Tensor, positions: Optional[torch.Tensor] = None,
+                   pending_residual: Optional[torch.Tensor] = None, defer_residual: bool = False):
+        """`decode` over a 4-bit cache: x [B, H], one token of every sequence into slot `lengths[b]` (int32 [B] on the
+        GPU; the caller advances it, an idle sequence has a negative one), rotated for `positions[b]` (int32 [B], the
+        lengths without it; they differ once a cache was cut).  Every launch is independent of both, so one captured graph
+        serves all steps.  Residuals are chained as in `decode_static`; the glue kernels always run."""
+        cfg = self.cfg
+        if pending_residual is not None:
+            h1, x = ops.rms_norm(x, self.norm1, cfg.eps, residual=pending_residual)
+        else:
+            h1 = ops.rms_norm(x, self.norm1, cfg.eps)
+        qkv = self._column_parallel_decode(h1, self.w_qkv, True)
+        ops.rope_axes_(qkv, self.hq + self.hkv, cfg.head_dim, lengths if positions is None else positions, (cfg.head_dim // 2,),
+                       cfg.rope_theta)
+        attn = ops.kv4_decode_attention_(qkv, cache, self.hq, lengths)
+        return self._decode_mlp(x, self._row_parallel_decode(attn, "o", True), True, True, defer_residual)
+
+
 def decode_local(layers, caches, x: torch.Tensor, pos) -> Optional[torch.Tensor]:
     """A decode step of a world of one through `layers` as one persistent kernel (per eight layers), or None
     where the step has to be composed of single ops: with peers, without the glue kernels, off the GPU,
@@ -498,6 +536,85 @@ def new_kv_caches(layers, batch: int, max_seq: int) -> list:
     return [(torch.zeros(batch, max_seq, lyr.hkv, lyr.cfg.head_dim, dtype=torch.bfloat16, device=lyr.device),
              torch.zeros(batch, max_seq, lyr.hkv, lyr.cfg.head_dim, dtype=torch.bfloat16, device=lyr.device))
             for lyr in layers]
+
+
+def decode_kv4_through(layers, caches, x: torch.Tensor, lengths: torch.Tensor,
+                       positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One decode step through stacked layers over 4-bit caches; the residual add that closes a layer rides in the RMSNorm
+    kernel that opens the next."""
+    layers = list(layers)
+    h, pending = x, None
+    for i, (lyr, cache) in enumerate(zip(layers, caches)):
+        defer = i + 1 < len(layers)
+        out = lyr.decode_kv4(h, cache, lengths, positions, pending_residual=pending, defer_residual=defer)
+        h, pending = out if defer else (out, None)
+    return h
+
+
+def new_kv4_caches(layers, batch: int, max_seq: int, track_weights: bool = False) -> list:
+    """An empty `ops.Kv4Cache` per layer, for the kv heads of this rank."""
+    return [ops.Kv4Cache.new(batch, max_seq, lyr.hkv, lyr.cfg.head_dim, lyr.device, track_weights=track_weights) for lyr in layers]
+
+
+class Kv4Sequences:
+    """A batch of sequences over 4-bit caches: what `LlamaTPStack` keeps of them with `kv_bits=4`.  `lengths` (slots in
+    use) and `positions` (tokens seen), int32 [batch] on the GPU, advance with every step; with `use_graph` the step is
+    one captured CUDA graph.  A sequence is made idle by a negative length."""
+
+    def __init__(self, layers, batch: int, max_seq: int, track_weights: bool = False, use_graph: bool = True):
+        self.layers, self.max_seq = list(layers), int(max_seq)
+        first = self.layers[0]
+        dev = first.device
+        self.caches = new_kv4_caches(self.layers, batch, max_seq, track_weights)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.positions = torch.zeros(batch, dtype=torch.int32, device=dev)
+        self.graph = None
+        if use_graph:
+            self.x = torch.zeros(batch, first.cfg.hidden, dtype=torch.bfloat16, device=dev)
+            # first calls allocate workspaces and rendezvous: outside the capture, on a side stream
+            side = torch.cuda.Stream(dev)
+            side.wait_stream(torch.cuda.current_stream(dev))
+            with torch.cuda.stream(side):
+                self._run(self.x)
+            torch.cuda.current_stream(dev).wait_stream(side)
+            torch.cuda.synchronize(dev)
+            self.graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(self.graph):
+                self.y = self._run(self.x)
+            self.reset()
+
+    def _run(self, x: torch.Tensor) -> torch.Tensor:
+        y = decode_kv4_through(self.layers, self.caches, x, self.lengths, self.positions)
+        active = self.lengths >= 0
+        self.lengths += active
+        self.positions += active
+        return y
+
+    def reset(self) -> None:
+        """Start new sequences."""
+        for cache in self.caches:
+            cache.reset()
+        self.lengths.zero_()
+        self.positions.zero_()
+
+    def begin(self, seq: int) -> None:
+        """A prompt of `seq` tokens is in the caches."""
+        self.lengths.fill_(seq)
+        self.positions.fill_(seq)
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        """The next token of every sequence: [batch, H] in and out; with the graph the result is overwritten by the next step."""
+        if self.graph is None:
+            return self._run(x)
+        self.x.copy_(x)
+        self.graph.replay()
+        return self.y
+
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """Cut every layer's caches to `keep` slots a sequence (`ops.kv4_evict_`); positions go on counting tokens."""
+        for cache in self.caches:
+            lengths = ops.kv4_evict_(cache, self.lengths, keep, recent)
+        self.lengths.copy_(lengths)
 
 
 class DecodeGraph:
@@ -575,21 +692,38 @@ class LlamaTPStack:
         y_shard = stack.prefill(x_shard, seq=prompt_len)      # [batch * prompt_len / WS, H] in and out
         for pos in range(prompt_len, prompt_len + new_tokens):
             y = stack.decode_step(x, pos)                      # [batch, H] in and out, replicated on all ranks
+
+    With `kv_bits=4` the caches hold 4.5 bits a value (`stack.sequences`, a `Kv4Sequences`, has them with the sequences'
+    lengths and positions); with `track_weights` too, `stack.evict(keep, recent)` cuts them to the heaviest slots between two
+    steps.  `pos` is then the number of tokens before this one for all sequences, or None to go on from `sequences.positions`.
     """
 
     def __init__(self, cfg: LlamaTPConfig, n_layers: int, device: torch.device, batch: int, max_seq: int,
-                 group=None, seed: int = 0, use_graph: Optional[bool] = None, **layer_kwargs):
+                 group=None, seed: int = 0, use_graph: Optional[bool] = None, kv_bits: int = 16, track_weights: bool = False,
+                 **layer_kwargs):
+        if kv_bits not in (4, 16):
+            raise ValueError("kv_bits is 4 or 16")
+        if track_weights and kv_bits != 4:
+            raise ValueError("attention weights are tracked by 4-bit caches")
         self.cfg, self.batch, self.max_seq = cfg, int(batch), int(max_seq)
         self.layers = [LlamaTPDecoderLayer(cfg, device, group=group, seed=seed + 1000 * i, **layer_kwargs)
                        for i in range(n_layers)]
-        self.caches = new_kv_caches(self.layers, batch, max_seq)
         self.use_graph = (device.type == "cuda") if use_graph is None else bool(use_graph)
+        self.sequences = None
+        if kv_bits == 4:
+            self.sequences = Kv4Sequences(self.layers, batch, max_seq, track_weights, self.use_graph)
+            self.caches, self.graph = self.sequences.caches, self.sequences.graph
+            return
+        self.caches = new_kv_caches(self.layers, batch, max_seq)
         self._pos = torch.zeros(1, dtype=torch.int32, device=device)
         # built before any prefill: capturing runs warm-up steps that write into the caches
         self.graph = DecodeGraph(self.layers, batch, max_seq, caches=self.caches) if self.use_graph else None
 
     def reset(self) -> None:
         """Start new sequences: zero the caches."""
+        if self.sequences is not None:
+            self.sequences.reset()
+            return
         for kc, vc in self.caches:
             kc.zero_()
             vc.zero_()
@@ -602,11 +736,25 @@ class LlamaTPStack:
         h = x_shard
         for lyr, cache in zip(self.layers, self.caches):
             h = lyr.forward(h, self.batch, seq, kv_cache=cache)
+        if self.sequences is not None:
+            self.sequences.begin(seq)
         return h
 
-    def decode_step(self, x: torch.Tensor, pos: int) -> torch.Tensor:
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """Cut 4-bit caches that track weights to `keep` slots a sequence, between two steps."""
+        if self.sequences is None:
+            raise ValueError("eviction needs kv_bits=4 and track_weights")
+        self.sequences.evict(keep, recent)
+
+    def decode_step(self, x: torch.Tensor, pos: Optional[int] = None) -> torch.Tensor:
         """One token per sequence at position `pos`: [batch, H] in (replicated), [batch, H] out.  With
         the graph the result tensor is overwritten by the next step."""
+        if self.sequences is not None:
+            if pos is not None:
+                self.sequences.positions.fill_(pos)
+            return self.sequences.step(x)
+        if pos is None:
+            raise ValueError("pos is the token's position")
         if self.graph is not None:
             return self.graph.step(x, pos)
         if not 0 <= pos < self.max_seq:

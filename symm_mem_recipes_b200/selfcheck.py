@@ -246,6 +246,33 @@ def build_checks(world: int, rank: int, dev: torch.device) -> list:
 
     add("glue", "rms_norm / rope / silu_mul / decode_attention", glue, True)
 
+    def kv4():
+        cache = ops.Kv4Cache.new(2, 300, 1, 128, dev, track_weights=True)
+        k, v = randn(2, 257, 1, 128, std=0.7, seed=6), randn(2, 257, 1, 128, std=0.7, seed=7)
+        ops.kv4_append_(k, v, cache)
+        rk, rv = ops.kv4_read(cache, 257)
+        ok1 = bool(((rk - k).abs() <= 0.08 * k.abs().amax() + 1e-3).all()) and bool(((rv - v).abs() <= 0.08 * v.abs().amax() + 1e-3).all())
+        step = randn(2, (8 + 2) * 128, std=0.7, seed=8)
+        lengths = torch.tensor([257, 257], dtype=torch.int32, device=dev)
+        got = ops.kv4_decode_attention_(step, cache, 8, lengths)
+        wk, wv = ops.kv4_read(cache, 258)
+        q = step[:, : 8 * 128].view(2, 8, 1, 128).float()
+        p = torch.softmax(q @ wk.float().permute(0, 2, 3, 1) / 128 ** 0.5, dim=-1)
+        ref = (p @ wv.float().transpose(1, 2)).reshape(2, 8 * 128)
+        ok2 = _close(got, ref, 2.0 ** -6, 4e-3)[0]
+        ok3 = bool((cache.weights[:, 0, :258] - p.sum(1)[:, 0]).abs().max() < 1e-2)
+        new = ops.kv4_evict_(cache, lengths + 1, 100, recent=10)
+        ok4 = new.tolist() == [100, 100] and bool((cache.weights[:, 0, :90].amin(1) >= 0).all())
+        x = randn(3, 3 * 128, std=0.7, seed=9)
+        y = ops.rope_axes_(x.clone(), 2, 128, torch.tensor([[5, 9, 100000]] * 3, dtype=torch.int32, device=dev), (16, 24, 24), 5e5)
+        back = ops.rope_axes_(y.clone(), 2, 128, torch.tensor([[5, 9, 100000]] * 3, dtype=torch.int32, device=dev), (16, 24, 24), 5e5,
+                              inverse=True)
+        ok5 = _close(back, x, 2.0 ** -6, 2.0 ** -6)[0] and not torch.equal(y, x)
+        symm_mem.check_status(dev)
+        return ok1 and ok2 and ok3 and ok4 and ok5, f"append {ok1}, attention {ok2}, weights {ok3}, evict {ok4}, rope_axes {ok5}"
+
+    add("glue", "4-bit KV cache, rotation by axes", kv4, True)
+
     def layer(kind, fused_glue=False, fused_swiglu=False):
         def fn():
             cfg = LlamaTPConfig.tiny(world)

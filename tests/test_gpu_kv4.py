@@ -512,3 +512,72 @@ def test_serving_run(hkv, g, dim):
         if step == 7:
             check_evict(cache, lengths.tolist(), 40, 8)
             lengths = lengths.clamp(max=40)
+
+
+# ---- the layer and the stack ----
+
+def stack_of(**kw):
+    from symm_mem_recipes_b200.models.llama_tp_layer import LlamaTPConfig, LlamaTPStack
+    cfg = LlamaTPConfig(hidden=512, n_heads=8, n_kv_heads=2, head_dim=64, ffn=512)
+    return LlamaTPStack(cfg, 2, torch.device("cuda", torch.cuda.current_device()), batch=3, max_seq=96, seed=3, **kw)
+
+
+def test_stack_with_a_4_bit_cache():
+    """A prompt and steps through two layers: the graph's steps are the eager ones, a step is what its ops make of it one by one,
+    and the prompt's rows are in the caches as `kv4_append_` puts them there."""
+    from symm_mem_recipes_b200.models.llama_tp_layer import new_kv_caches
+    graph, eager = stack_of(kv_bits=4, track_weights=True), stack_of(kv_bits=4, track_weights=True, use_graph=False)
+    plain = stack_of(use_graph=False)
+    x = normal(70, 3 * 40, 512, std=0.5)
+    y = graph.prefill(x, 40)
+    assert torch.equal(y, eager.prefill(x, 40)) and torch.equal(y, plain.prefill(x, 40))
+    for cache, (kc, vc) in zip(graph.caches, plain.caches):
+        want = ops.Kv4Cache.new(3, 96, 2, 64, "cuda", track_weights=True)
+        ops.kv4_append_(kc[:, :40], vc[:, :40], want)
+        assert same(cache, want)
+    assert graph.sequences.lengths.tolist() == [40] * 3
+    far = 0.0
+    for step in range(6):
+        x = normal(80 + step, 3, 512, std=0.5)
+        manual = [copy_of(c) for c in eager.caches]
+        lengths, positions = eager.sequences.lengths.clone(), eager.sequences.positions.clone()
+        a, b = graph.decode_step(x).clone(), eager.decode_step(x)
+        assert torch.equal(a, b)
+        h = x
+        for lyr, cache in zip(eager.layers, manual):
+            qkv = ops.gemv(ops.rms_norm(h, lyr.norm1, lyr.cfg.eps), lyr.w_qkv, weights_nk=True)
+            ops.rope_axes_(qkv, lyr.hq + lyr.hkv, 64, positions, (32,), lyr.cfg.rope_theta)
+            out = ops.kv4_decode_attention_(qkv, cache, lyr.hq, lengths)
+            h2, x1 = ops.rms_norm(lyr._row_parallel_decode(out, "o", True), lyr.norm2, lyr.cfg.eps, residual=h)
+            h = x1 + lyr._row_parallel_decode(ops.silu_mul(ops.gemv(h2, lyr.w_gate_up, weights_nk=True)), "down", True)
+        assert torch.equal(h, b) and all(same(m, c) for m, c in zip(manual, eager.caches))
+        assert torch.isfinite(a).all()
+        ref16 = plain.decode_step(x, 40 + step)
+        far = max(far, float((a.double() - ref16.double()).norm() / ref16.double().norm()))
+    assert far < 1.0        # four bits instead of sixteen, not another function
+    graph.evict(30, recent=4)
+    assert graph.sequences.lengths.tolist() == [30] * 3 and graph.sequences.positions.tolist() == [46] * 3
+    graph.sequences.lengths[1] = -1
+    before = [copy_of(c) for c in graph.caches]
+    y = graph.decode_step(normal(90, 3, 512, std=0.5))
+    assert torch.isfinite(y).all() and graph.sequences.lengths.tolist() == [31, -1, 31]
+    assert graph.sequences.positions.tolist() == [47, 46, 47]
+    for was, now in zip(before, graph.caches):
+        assert torch.equal(was.k_codes[1], now.k_codes[1]) and torch.equal(was.weights[1], now.weights[1])
+    graph.reset()
+    assert not graph.caches[0].weights.any() and graph.sequences.lengths.tolist() == [0] * 3
+    assert len(new_kv_caches(plain.layers, 1, 4)) == 2
+
+
+def test_stack_refuses():
+    with pytest.raises(ValueError, match="kv_bits"):
+        stack_of(kv_bits=8)
+    with pytest.raises(ValueError, match="4-bit"):
+        stack_of(track_weights=True)
+    plain = stack_of(use_graph=False)
+    with pytest.raises(ValueError, match="kv_bits=4"):
+        plain.evict(3)
+    with pytest.raises(ValueError, match="position"):
+        plain.decode_step(torch.zeros(3, 512, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError, match="Kv4Cache of this batch"):
+        plain.layers[0].forward(normal(1, 3 * 8, 512), 3, 8, kv_cache=ops.Kv4Cache.new(2, 96, 2, 64, "cuda"))
