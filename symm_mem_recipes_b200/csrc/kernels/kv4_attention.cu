@@ -920,6 +920,19 @@ __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const _
     if (t < n) fetch_tile<D, false>(a.cache, base + (size_t)t * kTile, ring_addr + i * L::kBytes);
     copy_commit();
   }
+  // the weights so far, of this lane's two slots a tile, come in meanwhile
+  float* weights = kScores ? a.cache.weights + base : nullptr;
+  float so_far[kScores ? kHeadTiles : 1][kTile / 32];
+  if constexpr (kScores) {
+#pragma unroll
+    for (int i = 0; i < kHeadTiles; ++i) {
+#pragma unroll
+      for (int k = 0; k < kTile / 32; ++k) {
+        const int slot = (first + i * step) * kTile + k * 32 + lane;
+        so_far[i][k] = slot < len ? weights[slot] : 0.0f;      // the new token's starts from zero
+      }
+    }
+  }
   Attend<D, kScores> at;
   at.start(a, b, h);
   for (int t = first, i = 0; t < n; t += step, ++i) {
@@ -975,38 +988,42 @@ __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const _
       join_pieces<kHeadCtas>(
           ctas, [&](int i, int what) { return load_remote(remote_of(cta_piece + what * kHeads + q, i)); },
           [&](int i) { return load_remote_4(remote_of(cta_piece + 2 * kHeads + q * D + 4 * d, i)); }, m, l, o);
+  } else {
+    __syncthreads();      // cta_piece is read by other threads than it was written by
   }
   if (mine) {
     const float inv = 1.0f / l;
     *reinterpret_cast<uint2*>(out + q * D + 4 * d) = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
   }
   if constexpr (kScores) {
-    if (tid < a.group) {
+    if (warp == kHeadWarps - 1 && lane < a.group) {      // a warp that has joined few heads or none
       float4 none;
       if (ctas > 1)
         join_pieces<kHeadCtas>(
-            ctas, [&](int i, int what) { return load_remote(remote_of(cta_piece + what * kHeads + tid, i)); },
+            ctas, [&](int i, int what) { return load_remote(remote_of(cta_piece + what * kHeads + lane, i)); },
             [&](int) { return make_float4(0.0f, 0.0f, 0.0f, 0.0f); }, m, l, none);
       else
-        m = cta_piece[tid], l = cta_piece[kHeads + tid];
-      norms[0][tid] = m;
-      norms[1][tid] = 1.0f / l;
+        m = cta_piece[lane], l = cta_piece[kHeads + lane];
+      norms[0][lane] = m;
+      norms[1][lane] = 1.0f / l;
     }
   }
   __syncwarp();
   if (ctas > 1) cluster_arrive();      // nothing of another CTA's is read from here on
   if constexpr (kScores) {
     __syncthreads();
-    float* weights = a.cache.weights + base;
-    for (int t = first, i = 0; t < n; t += step, ++i) {
+#pragma unroll
+    for (int i = 0; i < kHeadTiles; ++i) {
 #pragma unroll
       for (int k = 0; k < kTile / 32; ++k) {
-        const int slot = t * kTile + k * 32 + lane;
+        const int slot = (first + i * step) * kTile + k * 32 + lane;
         if (slot > len) continue;
         const float* s = scores + (i * kTile + k * 32 + lane) * pitch;
         float p = 0.0f;
-        for (int j = 0; j < a.group; ++j) p += exp2_of(s[j] - norms[0][j]) * norms[1][j];
-        weights[slot] = slot == len ? p : weights[slot] + p;
+#pragma unroll
+        for (int j = 0; j < kHeads; ++j)
+          if (j < a.group) p += exp2_of(s[j] - norms[0][j]) * norms[1][j];
+        weights[slot] = so_far[i][k] + p;
       }
     }
   }
