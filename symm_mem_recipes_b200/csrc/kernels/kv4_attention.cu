@@ -26,6 +26,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../device/pdl.cuh"
 #include "kv4.cuh"
@@ -1031,14 +1032,53 @@ __global__ void __launch_bounds__(32 * kHeadWarps, 1) attend_head_kernel(const _
   if (ctas > 1) cluster_wait();
 }
 
-// CTAs a head of the kernel above, or 0 where it does not take the call: heads of more slots than it has room for, or more heads
-// than a wave of CTAs (148 SMs hold sixteen clusters of eight).
+template <int D>
+constexpr size_t head_smem(int tiles_a_warp, int score_pitch) {      // pitch 0: no scores
+  return kHeadWarps * ((size_t)kHeadStages * Layout<D>::kBytes + (size_t)tiles_a_warp * kTile * score_pitch * sizeof(float));
+}
+
+// Clusters of `ctas` of the kernel's largest CTAs that the current device holds at once, asked once per device: SMs are grouped,
+// and a group holds whole clusters (148 SMs: 15 of eight, 22 of six, 33 of four).
+int resident_clusters(int ctas) {
+  constexpr int kDevices = 64;
+  static std::atomic<int> known[kDevices][kHeadCtas + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kDevices) return 0;
+  int n = known[dev][ctas].load(std::memory_order_relaxed);
+  if (n > 0) return n - 1;
+  const auto kernel = attend_head_kernel<128, true>;
+  const size_t smem = head_smem<128>(kHeadTiles, kHeads);
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ctas;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(32 * kHeadWarps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int clusters = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) != cudaSuccess) {
+    (void)cudaGetLastError();
+    clusters = 0;
+  }
+  known[dev][ctas].store(clusters + 1, std::memory_order_relaxed);
+  return clusters;
+}
+
+// CTAs a head of the kernel above, or 0 where it does not take the call: as many as there is work and room for at once, and
+// slots that they hold; without clusters up to two CTAs an SM one after the other.  Microseconds of one launch and of two, heads x slots
+// (0.3 to all of them in use, with weights):
+//     1 x 4096     8.1   9.8  |  64 x 2048  11.4  18.3  |  128 x 2048  15.9  25.7  |  256 x 1024  19.3  23.0
+//     256 x 2048  31.4  31.0  |  512 x 512  25.1  23.9  |  16 x 8192 with sixteen clusters of eight, which do not fit, 21.0  16.7
 int head_ctas(const Kv4Cache& cache, int batch, int num_sms) {
   const long long heads = (long long)batch * cache.hkv;
   const int tiles = cache.slots / kTile;
-  int ctas = 1;
-  while (ctas < kHeadCtas && 2 * ctas * heads * 8 <= 7ll * num_sms && ctas * kHeadWarps < tiles) ctas *= 2;
-  return heads <= num_sms && tiles <= ctas * kHeadWarps * kHeadTiles ? ctas : 0;
+  int ctas = std::max(1, std::min(kHeadCtas, (tiles + kHeadWarps - 1) / kHeadWarps));
+  while (ctas > 1 && heads > resident_clusters(ctas)) --ctas;
+  return heads <= (ctas == 1 ? 2 * num_sms : num_sms) && tiles <= ctas * kHeadWarps * kHeadTiles ? ctas : 0;
 }
 
 int attention_ctas(const Kv4Cache& cache, int batch, int num_sms) {
@@ -1071,8 +1111,7 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const int tiles = a.cache.slots / kTile;
   if (const int ctas = head_ctas(a.cache, a.batch, a.num_sms)) {
     const int a_warp = std::max(1, (tiles + ctas * kHeadWarps - 1) / (ctas * kHeadWarps));
-    const size_t smem = kHeadWarps * ((size_t)kHeadStages * Layout<D>::kBytes +
-                                      (kScores ? (size_t)a_warp * kTile * padded_group(a.group) * sizeof(float) : 0));
+    const size_t smem = head_smem<D>(a_warp, kScores ? padded_group(a.group) : 0);
     return launch_kernel(attend_head_kernel<D, kScores>, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), 32 * kHeadWarps, smem, ctas,
                          stream, a, ctas, a_warp);
   }
