@@ -31,8 +31,11 @@ __device__ __forceinline__ Vec16 pack8(const float (&f)[8]) {
   return o;
 }
 
-// A CTA takes `per` tokens: first the (cos, sin) of their D / 2 pairs, then the heads, eight pairs a thread and step.
-template <int D>
+// A CTA takes `per` tokens: first the (cos, sin) of their D / 2 pairs, then the heads, eight pairs a thread and step.  Bound by
+// HBM: 8192 tokens of 72 heads of 128 (302 MB read and written) 51.0 us, 91 % of the copy rate; several steps' loads in
+// flight at a time were slower (two 52, four 66).  kOnce: the result is more than L2 keeps, its lines are the first to
+// leave (53.3 us without).
+template <int D, bool kOnce>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int per) {
   constexpr int kPairs = D / 2, kVecs = D / 16;
   __shared__ __align__(16) float cosine[kMaxTokens * kPairs], sine[kMaxTokens * kPairs];
@@ -56,8 +59,8 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
     const int t = i / a.n_heads, h = i - t * a.n_heads;
     __nv_bfloat16* p = base + (size_t)t * a.row_stride + h * D;
     float x[8], y[8], u[8], v[8];
-    unpack8(ld_16(p), x);
-    unpack8(ld_16(p + kPairs), y);
+    unpack8(ld_16_stream(p), x);
+    unpack8(ld_16_stream(p + kPairs), y);
     const float* c = cosine + t * kPairs + vec * 8;
     const float* s = sine + t * kPairs + vec * 8;
 #pragma unroll
@@ -65,8 +68,13 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
       u[k] = x[k] * c[k] - y[k] * s[k];
       v[k] = y[k] * c[k] + x[k] * s[k];
     }
-    st_16(p, pack8(u));
-    st_16(p + kPairs, pack8(v));
+    if constexpr (kOnce) {
+      st_16_stream(p, pack8(u));
+      st_16_stream(p + kPairs, pack8(v));
+    } else {
+      st_16(p, pack8(u));
+      st_16(p + kPairs, pack8(v));
+    }
   }
 }
 
@@ -78,8 +86,10 @@ int launch_rope_axes(const RopeAxesArgs& a, cudaStream_t stream) {
   const int per = min(kMaxTokens, max(1, 1024 / items));
   const long long blocks = (a.tokens + per - 1) / per;
   if (blocks > 0x7fffffffll) return (int)cudaErrorInvalidValue;
-  if (a.head_dim == 128) rope_axes_kernel<128><<<(unsigned)blocks, kThreads, 0, stream>>>(a, per);
-  else rope_axes_kernel<64><<<(unsigned)blocks, kThreads, 0, stream>>>(a, per);
+  const bool once = a.tokens * a.n_heads * a.head_dim * 2 >= (64ll << 20);
+  const auto kernel = a.head_dim == 128 ? (once ? rope_axes_kernel<128, true> : rope_axes_kernel<128, false>)
+                                        : (once ? rope_axes_kernel<64, true> : rope_axes_kernel<64, false>);
+  kernel<<<(unsigned)blocks, kThreads, 0, stream>>>(a, per);
   return (int)cudaGetLastError();
 }
 
