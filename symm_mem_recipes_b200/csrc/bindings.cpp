@@ -22,6 +22,7 @@
 
 #include "kernels/decode_stack.h"
 #include "kernels/gemv_local.h"
+#include "kernels/kv4_shares.h"
 #include "kernels/launch.h"
 #include "oracle/cpu_reference.h"
 #include "symm/allocator.h"
@@ -818,6 +819,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 
   m.def("check_push_schedule", &check_push_schedule);
   m.def("check_pair_work", &check_pair_work);
+  m.def("check_kv4_cuts", [](const std::vector<int>& tiles, int ctas) { return check_kv4_cuts(tiles.data(), (int)tiles.size(), ctas); });
   m.def("check_wide_work", &check_wide_work);
   m.def("check_rs_pair_schedule", &check_rs_pair_schedule);
   m.def("check_rs_progress", &check_rs_progress);
@@ -1280,8 +1282,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     }
     need_per_sequence(start, k.size(0), "start");
     need_per_sequence(counts, k.size(0), "counts");
-    need(start.has_value() || (start0 >= 0 && start0 + k.size(1) <= max_seq), "slots [", start0, ", ", start0 + k.size(1),
-         ") are outside the cache of ", max_seq);
+    need(start.has_value() || (start0 >= 0 && start0 <= max_seq - k.size(1)), k.size(1), " tokens from slot ", start0,
+         " are outside the cache of ", max_seq);
     int64_t batch;
     a.cache = kv4_cache(kc, ks, vc, vs, weights, max_seq, &batch);
     const int dev = kc.get_device();

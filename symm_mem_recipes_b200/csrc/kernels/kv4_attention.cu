@@ -30,6 +30,7 @@
 
 #include "../device/pdl.cuh"
 #include "kv4.cuh"
+#include "kv4_shares.h"
 #include "launch.h"
 
 namespace smr {
@@ -38,7 +39,6 @@ namespace {
 
 using namespace kv4;
 
-constexpr int kWarps = 4;                 // of an attention CTA
 constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
 constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
 constexpr int kJoinThreads = 256;
@@ -76,18 +76,6 @@ __device__ __forceinline__ int tiles_of(const Kv4AttentionArgs& a, int b) {
   const int n = length_of(a, b);
   return n >= 0 && n < a.cache.max_seq ? n / kTile + 1 : 0;
 }
-// The list's tiles among the warps: the first `more` of them have one tile more than the others.  (One 32-bit division; with
-// tiles * w / warps in 64 bits the second kernel spent 20 us on divisions.)
-struct Shares {
-  int tiles, each, more;
-  __device__ __forceinline__ Shares(int tiles, int warps) : tiles(tiles), each(tiles / warps), more(tiles - each * warps) {}
-  __device__ __forceinline__ int first(int w) const { return w * each + min(w, more); }
-  __device__ __forceinline__ int warp_of(int tile) const {
-    const int of_more = more * (each + 1);
-    return tile < of_more ? tile / (each + 1) : more + (tile - of_more) / each;      // each > 0 where a tile is behind those
-  }
-};
-
 // kOnce: the lines are the first to leave L2, where others are wanted again.
 template <bool kOnce>
 __device__ __forceinline__ void copy_async_16(uint32_t dst, const void* src, uint64_t policy) {
@@ -137,14 +125,6 @@ __device__ __forceinline__ float exp2_of(float x) {
 }
 __device__ __forceinline__ float lo_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 << 16); }
 __device__ __forceinline__ float hi_of(uint32_t bf16x2) { return __uint_as_float(bf16x2 & 0xFFFF0000u); }
-
-// What a warp of the list ends with: a head that it does not finish by itself (sequence * kv heads + kv head).
-struct FinalPiece {
-  int head;
-  bool whole, last;      // has the head's first tile, its last one
-  int slot;              // of its two pieces' places
-};
-constexpr int kNoPiece = -1, kNoTiles = -2;
 
 // Where a warp is in the list of tiles.
 struct Cursor {
@@ -647,12 +627,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   for (int w0 = 0; w0 < kWarps; ++w0) {
     const FinalPiece lead = final_of[w0];
     if (lead.head < 0) continue;
-    int w1 = w0 + 1;
-    bool last = lead.last;
-    while (w1 < kWarps && (final_of[w1].head == lead.head || final_of[w1].head == kNoTiles)) {
-      if (final_of[w1].head == lead.head) last = final_of[w1].last;
-      ++w1;
-    }
+    bool last;
+    const int w1 = run_of(final_of, w0, last);
     constexpr int kSide = D / 4, kSides = 32 * kWarps / kSide;      // threads a query head, four dims each
     const int d = threadIdx.x % kSide;
     for (int q = threadIdx.x / kSide; q < a.group; q += kSides) {
@@ -684,28 +660,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   }
 }
 
-// The pieces of a head whose tiles are [s0, s1) of the list: one of every CTA that has some, at the first of its warps that does
-// (warps that ended in the head joined theirs), and one more of the last warp, where that went on to another head and is not
-// the first itself.
-template <int D>
-struct Pieces {
-  const Workspace& ws;
-  Shares shares;
-  int s0, wa, wb, ctas, count;
-  bool finished;      // by the first kernel
-  __device__ __forceinline__ Pieces(const Workspace& ws, int tiles, int warps, int s0, int s1)
-      : ws(ws), shares(tiles, warps), s0(s0), wa(shares.warp_of(s0)), wb(shares.warp_of(s1 - 1)) {
-    const int ca = wa / kWarps, cb = wb / kWarps;
-    const bool ends = shares.first(wb + 1) == s1;
-    ctas = cb - ca + 1;
-    count = ctas + (!ends && wb != max(wa, cb * kWarps) ? 1 : 0);
-    finished = wa == wb || (ca == cb && ends);
-  }
-  __device__ __forceinline__ const float* at(int k) const {
-    const int w = k == 0 ? wa : k < ctas ? (wa / kWarps + k) * kWarps : wb;
-    return ws.pieces + ((size_t)w * 2 + (shares.first(w) < s0 ? 1 : 0)) * Layout<D>::kPiece;
-  }
-};
 __device__ __forceinline__ void add_piece(float& m, float& l, float mi, float li) {
   const float top = fmaxf(m, mi);
   l = (m == -INFINITY ? 0.0f : exp2_of(m - top)) * l + (mi == -INFINITY ? 0.0f : exp2_of(mi - top)) * li;
@@ -717,6 +671,7 @@ __device__ __forceinline__ void add_piece(float& m, float& l, float mi, float li
 template <int D, bool kScores>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Kv4AttentionArgs a, int warps, int outputs,
                                                             int chunks) {
+  using L = Layout<D>;
   constexpr int kJoinWarps = kJoinThreads / 32, kSide = D / 4, kLanes = 32 / kSide;      // kLanes pieces side by side in a warp
   __shared__ int sums[2][kJoinWarps];
   __shared__ float norms[2][kHeads];
@@ -759,23 +714,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
   const int s0 = before * hkv + h * n;
   pdl_launch_dependents();
-  const Pieces<D> pieces(ws, all * hkv, warps, s0, s0 + n);
+  const HeadCut cut(Shares(all * hkv, warps), s0, s0 + n);
+  auto piece = [&](int k) -> const float* { return ws.pieces + (size_t)cut.place(k) * L::kPiece; };
 
   pdl_wait();
   if (chunk0 < 0) {
-    if (pieces.finished) return;
+    if (cut.finished) return;
     // kJoinWarps / per warps a query head, each every `sides`-th group of pieces; four dims a thread
     const int per = a.group / outputs, sides = kJoinWarps / per, q = blockIdx.y * per + warp / sides, side = warp % sides;
     const int d = lane % kSide;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (warp < per * sides) {
-      for (int k = lane; k < pieces.count; k += 32) m = fmaxf(m, pieces.at(k)[q]);      // first, so that every piece is scaled once
+      for (int k = lane; k < cut.count; k += 32) m = fmaxf(m, piece(k)[q]);      // first, so that every piece is scaled once
 #pragma unroll
       for (int k = 16; k > 0; k >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, k));
 #pragma unroll 4
-      for (int k = side * kLanes + lane / kSide; k < pieces.count; k += sides * kLanes) {
-        const float* p = pieces.at(k);
+      for (int k = side * kLanes + lane / kSide; k < cut.count; k += sides * kLanes) {
+        const float* p = piece(k);
         const float f = p[q] == -INFINITY ? 0.0f : exp2_of(p[q] - m);
         const float4 v = *reinterpret_cast<const float4*>(p + 2 * kHeads + q * D + 4 * d);
         l += f * p[kHeads + q];
@@ -827,12 +783,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     fetch(chunk0, x);
     if (warp < a.group) {      // a warp a query head
       float m = -INFINITY, l = 0.0f;
-      if (pieces.finished) {
+      if (cut.finished) {
         const float2 s = ws.stats[(size_t)bh * kHeads + warp];
         m = s.x;
         l = s.y;
       } else {
-        for (int k = lane; k < pieces.count; k += 32) add_piece(m, l, pieces.at(k)[warp], pieces.at(k)[kHeads + warp]);
+        for (int k = lane; k < cut.count; k += 32) add_piece(m, l, piece(k)[warp], piece(k)[kHeads + warp]);
 #pragma unroll
         for (int k = 16; k > 0; k >>= 1) {
           const float mi = __shfl_xor_sync(0xffffffffu, m, k), li = __shfl_xor_sync(0xffffffffu, l, k);

@@ -6,6 +6,7 @@
 #include <vector>
 
 #include "ag_matmul_common.cuh"
+#include "kv4_shares.h"
 #include "matmul_rs_common.cuh"
 
 namespace smr {
@@ -252,6 +253,90 @@ int check_rs_progress(int world_size, int blocks_per_rank, int n_tiles_n, int n_
   for (int r = 0; r < world_size; ++r)
     for (int pair = 0; pair < n_pairs; ++pair)
       if (pair + next[(size_t)r * n_pairs + pair] * n_pairs < total_tiles) return 1;
+  return 0;
+}
+
+// The first kernel's walk over its tiles, as it leaves pieces, against what the second one looks for.  Codes:
+//  1 a place is written twice   2 a head is finished twice, or by the first kernel and the second
+//  3 a piece is not where it is looked for, or of another head   4 the pieces of a head are not its tiles, each once
+int check_kv4_cuts(const int* tiles_of, int heads, int ctas) {
+  using namespace kv4;
+  std::vector<int> start(heads + 1, 0);
+  for (int i = 0; i < heads; ++i) start[i + 1] = start[i] + tiles_of[i];
+  const int tiles = start[heads], warps = ctas * kWarps;
+  if (tiles == 0) return 0;
+  const Shares shares(tiles, warps);
+  struct Left {
+    int head, from, to;
+  };
+  std::vector<Left> places(2 * warps, Left{-1, 0, 0});
+  std::vector<int> done(heads, 0);
+  for (int c = 0; c < ctas; ++c) {
+    FinalPiece final_of[kWarps];
+    Left held[kWarps];
+    for (int v = 0; v < kWarps; ++v) {
+      const int w = c * kWarps + v, first = shares.first(w), end = shares.first(w + 1);
+      final_of[v] = FinalPiece{first == end ? kNoTiles : kNoPiece, false, false, 0};
+      if (first == end) continue;
+      int head = 0;
+      while (start[head + 1] <= first) ++head;
+      bool first_head = true, whole = first == start[head];
+      int from = first;
+      for (int i = first; i < end; ++i) {
+        const bool last = i == start[head + 1] - 1;
+        if (!last && i + 1 < end) continue;
+        if (last && whole) {
+          if (done[head]++) return 2;
+        } else if (i + 1 < end) {
+          if (places[2 * w].head >= 0) return 1;
+          places[2 * w] = Left{head, from, i + 1};
+        } else {
+          final_of[v] = FinalPiece{head, whole, last, first_head ? 0 : 1};
+          held[v] = Left{head, from, i + 1};
+        }
+        first_head = false;
+        whole = true;
+        from = i + 1;
+        if (last)
+          do ++head;
+          while (head < heads && tiles_of[head] == 0);
+      }
+    }
+    for (int v = 0; v < kWarps; ++v) {
+      if (final_of[v].head < 0) continue;
+      bool last;
+      const int v1 = run_of(final_of, v, last);
+      Left all = held[v];
+      for (int k = v + 1; k < v1; ++k) {
+        if (final_of[k].head == kNoTiles) continue;
+        if (held[k].from != all.to) return 4;
+        all.to = held[k].to;
+      }
+      if (final_of[v].whole && last) {
+        if (done[all.head]++) return 2;
+      } else {
+        Left& to = places[2 * (c * kWarps + v) + final_of[v].slot];
+        if (to.head >= 0) return 1;
+        to = all;
+      }
+      v = v1 - 1;
+    }
+  }
+  for (int i = 0; i < heads; ++i) {
+    if (tiles_of[i] == 0) continue;
+    const HeadCut cut(shares, start[i], start[i + 1]);
+    if (cut.finished != (done[i] == 1)) return 2;
+    if (cut.finished) continue;
+    std::vector<int> seen(tiles_of[i], 0);
+    for (int k = 0; k < cut.count; ++k) {
+      const Left& p = places[cut.place(k)];
+      if (p.head != i) return 3;
+      for (int t = p.from; t < p.to; ++t)
+        if (t < start[i] || t >= start[i + 1] || seen[t - start[i]]++) return 4;
+    }
+    for (int n : seen)
+      if (n != 1) return 4;
+  }
   return 0;
 }
 

@@ -263,6 +263,7 @@ def test_decode_attention(dim, hkv, g, weights, lengths):
 @pytest.mark.parametrize("batch, hkv, g, dim, max_seq, least", [
     (1, 1, 8, 128, 20011, 20010), (2, 2, 4, 128, 9001, 1), (40, 2, 3, 64, 700, 0), (300, 1, 2, 64, 100, 0), (1, 8, 8, 64, 33000, 32000),
     (160, 1, 8, 128, 130, -9), (75, 2, 5, 128, 320, -40), (19, 8, 1, 64, 1000, 0), (3, 3, 7, 128, 5000, 0), (33, 2, 8, 128, 2048, 0),
+    (1024, 1, 4, 64, 64, -20), (1000, 1, 1, 128, 200, -50),
 ])
 def test_decode_attention_long_and_many(batch, hkv, g, dim, max_seq, least):
     """Contexts over many tiles and CTAs, batches over many warps, ragged lengths."""
@@ -379,6 +380,31 @@ def test_decode_attention_on_two_streams_and_in_graphs():
         graphs[1].replay()
     torch.cuda.synchronize()
     assert torch.equal(outs[0], wa) and torch.equal(outs[1], wb) and same(caches[0], ca) and same(caches[1], cb)
+
+
+def test_first_calls_in_a_capture():
+    """A process whose first calls are captured: what is looked up once is looked up then."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from symm_mem_recipes_b200 import ops
+cache = ops.Kv4Cache.new(3, 5000, 2, 128, "cuda", track_weights=True)
+x, n = torch.randn(3, 12 * 128, device="cuda").bfloat16(), torch.tensor([4000, 0, 77], dtype=torch.int32, device="cuda")
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    ops.rope_axes_(x, 10, 128, n, (64,), 1e4)
+    out = ops.kv4_decode_attention_(x, cache, 8, n)
+    new = ops.kv4_evict_(cache, n + 1, 50)
+y = x.clone()
+g.replay()
+torch.cuda.synchronize()
+fresh = ops.Kv4Cache.new(3, 5000, 2, 128, "cuda", track_weights=True)
+ops.rope_axes_(y, 10, 128, n, (64,), 1e4)
+want = ops.kv4_decode_attention_(y, fresh, 8, n)
+assert torch.equal(x, y) and torch.equal(out, want) and new.tolist() == [50, 1, 50]
+"""
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=200)
 
 
 def test_offsets_beyond_32_bits():

@@ -163,3 +163,16 @@ def test_nibbles_are_those_of_the_exact_quotient():
         num, den = mx * 2 ** (shift + 3), ms * 8                 # ceil(num / den - 1/2) = ceil((2 num - den) / (2 den))
         want = np.minimum(-((den - 2 * num) // (2 * den)), 7)
         assert np.array_equal(got[keep].astype(int), want[keep])
+
+
+def test_cut_heads_are_joined_whole():
+    """Every tile of every head reaches the output once, however the list of tiles falls on warps and CTAs."""
+    import random
+
+    from symm_mem_recipes_b200._ext import C
+    assert C.check_kv4_cuts([], 3) == 0 and C.check_kv4_cuts([0, 0], 3) == 0
+    assert C.check_kv4_cuts([2048] * 8, 296) == 0 and C.check_kv4_cuts([1] * 2400, 296) == 0 and C.check_kv4_cuts([9000], 296) == 0
+    for seed in range(4000):
+        rng = random.Random(seed)
+        heads = [rng.choice((0, 1, 1, 2, 3, rng.randint(1, 40))) for _ in range(rng.randint(1, 14))]
+        assert C.check_kv4_cuts(heads, rng.randint(1, 7)) == 0, (seed, heads)
