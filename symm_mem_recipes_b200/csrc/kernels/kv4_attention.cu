@@ -32,6 +32,7 @@
 #include "kv4.cuh"
 #include "kv4_shares.h"
 #include "launch.h"
+#include "pdl_launch.h"
 
 namespace smr {
 
@@ -1042,43 +1043,23 @@ int attention_ctas(const Kv4Cache& cache, int batch, int num_sms) {
   return (int)std::max<long long>(1, std::min<long long>(2ll * num_sms, (tiles + kWarps - 1) / kWarps));
 }
 
-template <class... Params, class... Args>
-int launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
-  if (smem > 0)
-    if (int e = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
-  cudaLaunchAttribute attrs[2] = {};
-  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[0].val.programmaticStreamSerializationAllowed = 1;
-  attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = cluster;
-  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attrs;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <int D, bool kScores>
 int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const int tiles = a.cache.slots / kTile;
   if (const int ctas = head_ctas(a.cache, a.batch, a.num_sms)) {
     const int a_warp = std::max(1, (tiles + ctas * kHeadWarps - 1) / (ctas * kHeadWarps));
     const size_t smem = head_smem<D>(a_warp, kScores ? padded_group(a.group) : 0);
-    return launch_kernel(attend_head_kernel<D, kScores>, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), 32 * kHeadWarps, smem, ctas,
+    return launch_pdl(attend_head_kernel<D, kScores>, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), 32 * kHeadWarps, smem, ctas,
                          stream, a, ctas, a_warp);
   }
   const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
   const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
-  if (int e = launch_kernel(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
+  if (int e = launch_pdl(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
   // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; the weights' CTAs fill the GPU once.
   const int heads = a.batch * a.cache.hkv, resident = 4 * a.num_sms;
   const int outputs = heads * a.group <= 2 * resident ? a.group : 1;
   const int chunks = kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, resident / heads)) : 0;
-  return launch_kernel(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
+  return launch_pdl(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
                        chunks);
 }
 

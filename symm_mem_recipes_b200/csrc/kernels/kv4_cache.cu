@@ -8,6 +8,8 @@
 #include "../device/pdl.cuh"
 #include "kv4.cuh"
 #include "launch.h"
+#include "pdl_launch.h"
+#include "residency.h"
 
 namespace smr {
 
@@ -365,42 +367,24 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_co
   }
 }
 
-template <class... Params, class... Args>
-int launch_kernel(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, Args... args) {
-  cudaLaunchAttribute attrs[2] = {};
-  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[0].val.programmaticStreamSerializationAllowed = 1;
-  attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = cluster;
-  attrs[1].val.clusterDim.y = attrs[1].val.clusterDim.z = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cfg.attrs = attrs;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Four rows a thread once that still gives every SM several CTAs.
 constexpr int kManyRows = 4;
 bool many_rows(long long rows, int batch, int head_dim) {
   const int step = 256 / (head_dim / 8);
-  return 2 * batch * rows / (step * kManyRows) >= 148 * 4;
+  return 2 * batch * rows / (step * kManyRows) >= 4 * device_sms();
 }
 
 template <int D, int kRows>
 int append(const Kv4AppendArgs& a, long long rows, cudaStream_t stream) {
   constexpr int kBlock = 256 / (D / 8) * kRows;
-  return launch_kernel(append_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), a.batch, 2), 256, 0, 1, stream, a,
+  return launch_pdl(append_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), a.batch, 2), 256, 0, 1, stream, a,
                        Divisor(a.cache.hkv, 256 / (D / 8)));
 }
 template <int D, int kRows>
 int read(const Kv4Cache& cache, int batch, int n, void* k_out, void* v_out, cudaStream_t stream) {
   constexpr int kBlock = 256 / (D / 8) * kRows;
   const long long rows = (long long)n * cache.hkv;
-  return launch_kernel(read_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), batch, 2), 256, 0, 1, stream, cache,
+  return launch_pdl(read_kernel<D, kRows>, dim3((unsigned)((rows + kBlock - 1) / kBlock), batch, 2), 256, 0, 1, stream, cache,
                        Divisor(cache.hkv, 256 / (D / 8)), n, k_out, v_out);
 }
 
@@ -431,8 +415,7 @@ int launch_kv4_evict(const Kv4EvictArgs& a, cudaStream_t stream) {
   const int cached = std::min(run, kEvictKeys);
   const size_t smem = std::max(cached * sizeof(uint32_t), a.cache.head_dim == 128 ? sizeof(EvictRows<128>) : sizeof(EvictRows<64>));
   auto kernel = a.cache.head_dim == 128 ? evict_kernel<128> : evict_kernel<64>;
-  if (int e = (int)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)) return e;
-  return launch_kernel(kernel, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), kEvictThreads, smem, ctas, stream, a, ctas, cached);
+  return launch_pdl(kernel, dim3((unsigned)(a.batch * a.cache.hkv * ctas)), kEvictThreads, smem, ctas, stream, a, ctas, cached);
 }
 
 }  // namespace smr

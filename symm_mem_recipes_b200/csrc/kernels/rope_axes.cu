@@ -10,6 +10,7 @@
 #include "../device/pdl.cuh"
 #include "../device/vec.cuh"
 #include "launch.h"
+#include "pdl_launch.h"
 
 namespace smr {
 
@@ -45,6 +46,7 @@ __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_consta
   const uint64_t frequency = a.frequency[pair];
   const int* pos = a.positions + (size_t)a.axis[pair] * a.position_stride + first;
   pdl_wait();
+  pdl_launch_dependents();
   for (int t = threadIdx.x / kPairs; t < tokens; t += kThreads / kPairs) {
     const uint64_t turns = frequency * (uint64_t)(int64_t)pos[t];
     float s, c;
@@ -89,8 +91,7 @@ int launch_rope_axes(const RopeAxesArgs& a, cudaStream_t stream) {
   const bool once = a.tokens * a.n_heads * a.head_dim * 2 >= (64ll << 20);
   const auto kernel = a.head_dim == 128 ? (once ? rope_axes_kernel<128, true> : rope_axes_kernel<128, false>)
                                         : (once ? rope_axes_kernel<64, true> : rope_axes_kernel<64, false>);
-  kernel<<<(unsigned)blocks, kThreads, 0, stream>>>(a, per);
-  return (int)cudaGetLastError();
+  return launch_pdl(kernel, dim3((unsigned)blocks), kThreads, 0, 1, stream, a, per);
 }
 
 }  // namespace smr
