@@ -247,6 +247,8 @@ def build_checks(world: int, rank: int, dev: torch.device) -> list:
     add("glue", "rms_norm / rope / silu_mul / decode_attention", glue, True)
 
     def kv4():
+        if not randn(1).is_cuda:
+            return True, "needs a GPU"
         cache = ops.Kv4Cache.new(2, 300, 1, 128, dev, track_weights=True)
         k, v = randn(2, 257, 1, 128, std=0.7, seed=6), randn(2, 257, 1, 128, std=0.7, seed=7)
         ops.kv4_append_(k, v, cache)
