@@ -47,7 +47,7 @@ using namespace kv4;
 constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
 constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
 constexpr int kJoinThreads = 256;
-constexpr int kJoinTiles = 8;             // tiles whose weights a CTA of the second kernel accumulates at a time
+constexpr int kJoinTiles = 16;             // tiles whose weights a CTA of the second kernel accumulates at a time
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -806,6 +806,12 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       }
     }
     __syncthreads();
+    float top[kHeads], inv[kHeads];
+#pragma unroll
+    for (int j = 0; j < kHeads; ++j) {      // a head that is not there adds nothing
+      top[j] = j < a.group ? norms[0][j] : 0.0f;
+      inv[j] = j < a.group ? norms[1][j] : 0.0f;
+    }
     for (int chunk = chunk0; chunk * kJoinTiles < n; chunk += chunks) {
       Mine ahead;
       fetch(chunk + chunks, ahead);
@@ -816,8 +822,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
         float p = 0.0f;
 #pragma unroll
         for (int j = 0; j < kHeads / 2; ++j) {
-          if (2 * j < a.group) p += exp2_of(x.s[k][j].x - norms[0][2 * j]) * norms[1][2 * j];
-          if (2 * j + 1 < a.group) p += exp2_of(x.s[k][j].y - norms[0][2 * j + 1]) * norms[1][2 * j + 1];
+          if (2 * j < a.group) p = fmaf(exp2_of(x.s[k][j].x - top[2 * j]), inv[2 * j], p);
+          if (2 * j + 1 < a.group) p = fmaf(exp2_of(x.s[k][j].y - top[2 * j + 1]), inv[2 * j + 1], p);
         }
         weights[i] = i == len ? p : x.weight[k] + p;
       }
@@ -1060,8 +1066,8 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
   if (int e = launch_pdl(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
   // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; the weights' CTAs fill the GPU once.
-  const int heads = a.batch * a.cache.hkv, resident = 4 * a.num_sms;
-  const int outputs = heads * a.group <= 2 * resident ? a.group : 1;
+  const int heads = a.batch * a.cache.hkv, resident = 2 * a.num_sms;
+  const int outputs = heads * a.group <= 4 * resident ? a.group : 1;
   const int chunks = kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, resident / heads)) : 0;
   return launch_pdl(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
                        chunks);
