@@ -23,7 +23,7 @@
 // S^T's accumulators hold heads in rows of four lanes, the second MMA wants keys there: movmatrix transposes in registers.
 //
 // Measured: 1.67 us per 1000 tiles at D = 128 (5.5 TB/s, 84 % of the copy rate) and 16 us besides; 32 x 8 heads of 6600 to 16384 slots
-// 103 us, 8 heads of 131072 with weights 56.  Reading alone takes 72 of the 103, computing alone 80: neither memory nor one
+// 103 us, 8 heads of 131072 with weights 53.  Reading alone takes 72 of the 103, computing alone 80: neither memory nor one
 // pipe is full (issue 52 %, ALU 51 %, tensor 32 %).  Three CTAs an SM, bulk copies and one stage less are no faster.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -835,7 +835,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
 // ---- one launch for caches of up to 2048 slots a head and CTA ----
 // A cluster of C CTAs takes a head, tile i the warp i % (8 C).  The warps' pieces meet in shared memory, the CTAs' over
 // distributed shared memory, and the scores wait in shared memory for their maxima and sums: no scratch, no second kernel.
-// 16 heads of up to 8192 with weights: 14.0 us, 18.5 as two launches.  A tile takes a warp 1.85 us with another on its scheduler.
+// 16 heads of 5300 to 8192 slots with weights: 14.3 us, 16.7 as two launches.  A tile takes a warp 1.85 us with another on its
+// scheduler.
 constexpr int kHeadWarps = 8;
 constexpr int kHeadTiles = 4;        // of a warp at most
 constexpr int kHeadStages = 2;

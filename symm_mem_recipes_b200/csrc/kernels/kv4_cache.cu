@@ -52,8 +52,9 @@ struct Row {
 // D / 8 lanes take a row of keys or of values, eight dims a lane, kRows rows a thread one after the other: their loads are in
 // flight together.  blockIdx.y is the sequence, blockIdx.z keys or values; row i of a sequence is head i % hkv of token i / hkv.
 // 2 bytes a value on one side, 0.56 on the other: 16384 tokens of 8 heads of 128 go in in 19 us and come back in 15, 34 together
-// where the bytes take 26 at the copy rate.  What goes in is bound by instruction issue (78 % of the slots, 120 instructions a
-// warp and two rows; 41 us with a 64-bit division for the row and an IEEE division for the scale).  Two rows a thread at a time 35, eight 38.
+// where the bytes take 26 at the copy rate; the rest is two launches that fill and drain.  (57 us with a 64-bit division for
+// the row and an IEEE division and a comparison a value.)  Two rows a thread at a time 35, eight 38; half a group a lane, which
+// halves the instructions, and tokens before heads, which makes a CTA's side of the cache one run of memory, 33 to 36.
 template <int D, int kRows, bool kValue>
 __device__ __forceinline__ void append_rows(const Kv4AppendArgs& a, const Divisor& hkv) {
   constexpr int kLanes = D / 8, kStep = 256 / kLanes;

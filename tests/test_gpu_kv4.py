@@ -197,6 +197,19 @@ def test_append_values_of_every_kind():
     assert nan.nonzero().tolist() == [[3, 0], [4, 1], [7, 1]]
 
 
+def test_append_from_an_int_and_unlike_strides():
+    """One start for all; keys contiguous, values a transposed view."""
+    cache, want = filled(16, 2, 90, 3, 128, weights=True), None
+    want = copy_of(cache)
+    k, v = normal(17, 2, 4, 3, 128), normal(18, 2, 3, 4, 128).transpose(1, 2)
+    for b in range(2):
+        for t in range(4):
+            put(want, b, 86 + t, k[b, t], v[b, t])
+            want.weights[b, :, 86 + t] = 0
+    ops.kv4_append_(k, v, cache, 86)
+    assert same(cache, want)
+
+
 def test_append_outside_is_skipped():
     """A start from the device that leaves the cache writes only what is inside."""
     cache = filled(13, 4, 70, 2, 64)
@@ -538,6 +551,37 @@ def test_serving_run(hkv, g, dim):
         if step == 7:
             check_evict(cache, lengths.tolist(), 40, 8)
             lengths = lengths.clamp(max=40)
+
+
+@pytest.mark.parametrize("batch, hkv, max_seq", [(3, 2, 700), (160, 1, 300), (2, 4, 21000)])
+def test_steps_back_to_back_are_the_steps_one_by_one(batch, hkv, max_seq):
+    """Launches that start under their predecessors: a chain of steps without a pause gives the bits of one with pauses."""
+    g, dim, keep = 4, 128, max_seq // 3
+    results = []
+    for pause in (True, False):
+        cache = filled(91, batch, max_seq, hkv, dim, weights=True)
+        lengths = torch.randint(0, max_seq - 10, (batch,), generator=gen(92), device="cuda").int()
+        outs = []
+        for step in range(8):
+            x = normal(93 + step, batch, (g + 2) * hkv * dim)
+            if pause:
+                torch.cuda.synchronize()
+            ops.rope_axes_(x, (g + 1) * hkv, dim, lengths, (64,), 1e4)
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(ops.kv4_decode_attention_(x, cache, g * hkv, lengths))
+            if pause:
+                torch.cuda.synchronize()
+            lengths = lengths + 1
+            if step % 3 == 2:
+                lengths = ops.kv4_evict_(cache, lengths, keep, recent=5)
+            if pause:
+                torch.cuda.synchronize()
+            k, v = ops.kv4_read(cache, 33)
+            ops.kv4_append_(v[:, :2], k[:, 3:5], cache, 7)
+        results.append((torch.stack(outs), cache))
+    torch.cuda.synchronize()
+    assert torch.equal(results[0][0], results[1][0]) and same(results[0][1], results[1][1])
 
 
 # ---- the layer and the stack ----
