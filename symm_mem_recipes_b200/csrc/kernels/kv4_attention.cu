@@ -47,7 +47,7 @@ using namespace kv4;
 constexpr int kHeads = 8;                 // query heads a kv head at most, the MMA's N
 constexpr int kRing = 27648;              // bytes of a warp's ring: two CTAs an SM
 constexpr int kJoinThreads = 256;
-constexpr int kJoinTiles = 16;             // tiles whose weights a CTA of the second kernel accumulates at a time
+constexpr int kJoinTiles = 4;             // tiles whose weights a CTA of the second kernel accumulates at a time: a slot a thread
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int D>
@@ -1066,12 +1066,14 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
   const int ctas = attention_ctas(a.cache, a.batch, a.num_sms);
   const size_t smem = kWarps * kRing + (size_t)(a.batch + 1) * sizeof(int);
   if (int e = launch_pdl(attend_kernel<D, kScores>, dim3(ctas), 32 * kWarps, smem, 1, stream, a)) return e;
-  // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; the weights' CTAs fill the GPU once.
-  const int heads = a.batch * a.cache.hkv, resident = 2 * a.num_sms;
-  const int outputs = heads * a.group <= 4 * resident ? a.group : 1;
-  const int chunks = kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, resident / heads)) : 0;
+  // A CTA a query head where there are few heads, whose pieces are many, else one a kv head; for the weights four CTAs an SM in all.
+  // In us, heads x slots, with a slot a thread, two and four (and two CTAs an SM): 8 x 131072 53.0, 54.0, 53.2; 320 x 8192 84.1, 86.7, 87.5;
+  // 1024 x 512 36.1, 37.7, 42.8.
+  const int heads = a.batch * a.cache.hkv, outputs = heads * a.group <= 8 * a.num_sms ? a.group : 1;
+  const int chunks =
+      kScores ? std::max(1, std::min((tiles + kJoinTiles - 1) / kJoinTiles, (4 * a.num_sms + heads - 1) / heads)) : 0;
   return launch_pdl(join_kernel<D, kScores>, dim3(heads, outputs + chunks), kJoinThreads, 0, 1, stream, a, ctas * kWarps, outputs,
-                       chunks);
+                    chunks);
 }
 
 }  // namespace
