@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Ca
 // to the lower slot.  The kept rows move down in slot order.  A cluster of C CTAs takes a head, each a run of its slots:
 //   1. a radix selection over the weights as ordered integers (kept in shared memory, so weights are read once) finds the
 //      weight of the last one kept, eight bits a pass; the CTAs' counts meet over distributed shared memory;
-//   2. warps count what stays of their own runs, the counts give every kept slot its place, and the places' sources are listed;
+//   2. the CTAs' counts of the passes and the warps' of their own runs give every kept slot its place, and the places' sources
+//      are listed;
 //   3. rows move in chunks of places, through shared memory by asynchronous copies (in registers 2048 rows of a cluster spilled
 //      and took 28 us of a prompt's 50).  A chunk is read whole before any of it is written; a place is never above its source
 //      and sources increase, so a chunk's writes cannot reach the sources of a later one.
@@ -194,8 +195,8 @@ template <int N>
 __device__ __forceinline__ void copy_async(void* dst, const void* src) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(smem_u32(dst)), "l"(src), "n"(N) : "memory");
 }
-// Sum of an integer in shared memory over the cluster's first `ctas` CTAs; the loads are in flight together.
-__device__ __forceinline__ int sum_over_ctas(const int* local, int ctas) {
+// Sums of an integer in shared memory over the cluster's first `mine` and `ctas` CTAs; the loads are in flight together.
+__device__ __forceinline__ int2 sum_over_ctas(const int* local, int mine, int ctas) {
   int v[kEvictCtas];
 #pragma unroll
   for (int r = 0; r < kEvictCtas; ++r) {
@@ -206,9 +207,12 @@ __device__ __forceinline__ int sum_over_ctas(const int* local, int ctas) {
       asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v[r]) : "r"(remote) : "memory");
     }
   }
-  int sum = 0;
+  int2 sum = make_int2(0, 0);
 #pragma unroll
-  for (int r = 0; r < kEvictCtas; ++r) sum += v[r];
+  for (int r = 0; r < kEvictCtas; ++r) {
+    sum.x += r < mine ? v[r] : 0;
+    sum.y += v[r];
+  }
   return sum;
 }
 __device__ __forceinline__ void cluster_barrier() {
@@ -221,10 +225,9 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_co
   pdl_wait();
   extern __shared__ __align__(16) uint32_t keys[];   // [cached], then EvictRows
   __shared__ int hist[2][256];                       // two passes in turn: one barrier a pass
-  __shared__ int total[256];
-  __shared__ int counts[2];                          // of this CTA: slots above the last worth kept, slots equal to it
+  __shared__ int2 total[256];                        // counts of the CTAs in front of this one, and of all
   __shared__ int warp_counts[2][kEvictWarps];
-  __shared__ int found[2];
+  __shared__ int found[4];                           // the digit, how many are left, and in front of this CTA: above it, with it
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.x / ctas, cta = blockIdx.x % ctas, b = head / a.cache.hkv;
   const int n = a.lengths[b], keep = a.keep;
@@ -244,6 +247,7 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_co
 
   uint32_t prefix = 0, mask = 0;
   int left = keep;                                   // slots still to be found among those that match the prefix
+  int above_before = 0, equal_before = 0;            // in front of this CTA's run: slots of more worth, slots that match
 #pragma unroll 1
   for (int pass = 0; pass < 4; ++pass) {
     const int shift = 24 - 8 * pass;
@@ -255,35 +259,48 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_co
     if (ctas > 1) cluster_barrier();
     else __syncthreads();
     if (tid < 256) {
-      total[tid] = ctas == 1 ? bins[tid] : sum_over_ctas(&bins[tid], ctas);
+      total[tid] = ctas == 1 ? make_int2(0, bins[tid]) : sum_over_ctas(&bins[tid], cta, ctas);
       if (pass > 0) hist[(pass + 1) & 1][tid] = 0;   // the last pass's, which nobody reads any more
     }
     __syncthreads();
     if (warp == 0) {      // a lane has eight bins, from the top down
-      int v[8], sum = 0;
+      int2 v[8], sum = make_int2(0, 0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += v[i] = total[255 - 8 * lane - i];
-      int before = sum;
+      for (int i = 0; i < 8; ++i) {
+        v[i] = total[255 - 8 * lane - i];
+        sum.x += v[i].x;
+        sum.y += v[i].y;
+      }
+      int2 before = sum;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += y;
+        const int x = __shfl_up_sync(0xffffffffu, before.x, o), y = __shfl_up_sync(0xffffffffu, before.y, o);
+        if (lane >= o) {
+          before.x += x;
+          before.y += y;
+        }
       }
-      before -= sum;
-      if (before < left && before + sum >= left) {
+      before.x -= sum.x;
+      before.y -= sum.y;
+      if (before.y < left && before.y + sum.y >= left) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          if (before < left && before + v[i] >= left) {
+          if (before.y < left && before.y + v[i].y >= left) {
             found[0] = 255 - 8 * lane - i;
-            found[1] = left - before;
+            found[1] = left - before.y;
+            found[2] = before.x;
+            found[3] = v[i].x;
           }
-          before += v[i];
+          before.x += v[i].x;
+          before.y += v[i].y;
         }
       }
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     left = found[1];
+    above_before += found[2];
+    equal_before = found[3];
     mask |= 255u << shift;
   }
   // `prefix` is the least worth that stays, of which the first `left` slots do
@@ -299,16 +316,7 @@ __global__ void __launch_bounds__(kEvictThreads, 4) evict_kernel(const __grid_co
     warp_counts[1][warp] = equal;
   }
   __syncthreads();
-  if (tid < 2) {
-    int sum = 0;
-    for (int i = 0; i < kEvictWarps; ++i) sum += warp_counts[tid][i];
-    counts[tid] = sum;
-  }
-  if (ctas > 1) cluster_barrier();
-  else __syncthreads();
-  // slots above and equal in front of this warp's run
-  int above_before = sum_over_ctas(&counts[0], cta), equal_before = sum_over_ctas(&counts[1], cta);
-  for (int i = 0; i < warp; ++i) {
+  for (int i = 0; i < warp; ++i) {                   // and in front of this warp's
     above_before += warp_counts[0][i];
     equal_before += warp_counts[1][i];
   }
