@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256) read_kernel(const __grid_constant__ Kv4Ca
 //   3. rows move in chunks of places, through shared memory by asynchronous copies (in registers 2048 rows of a cluster spilled
 //      and took 28 us of a prompt's 50).  A chunk is read whole before any of it is written; a place is never above its source
 //      and sources increase, so a chunk's writes cannot reach the sources of a later one.
-// 64 heads of up to 32768 to 4096 slots take 44 us: 3 for the weights, 2.3 a pass (a cluster barrier and remote loads), 5 for counts and
+// 64 heads of up to 32768 to 4096 slots take 43 us: 3 for the weights, 2.3 a pass (a cluster barrier and remote loads), 4 for counts and
 // list, 16 for the rows.
 constexpr int kEvictThreads = 256;
 constexpr int kEvictWarps = kEvictThreads / 32;
