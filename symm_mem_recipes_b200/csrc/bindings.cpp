@@ -361,6 +361,7 @@ Kv4Cache kv4_cache(const torch::Tensor& kc, const torch::Tensor& ks, const torch
          s->size(2) == slots && s->size(3) == D / 32, "scales must be bfloat16 [batch, kv heads, slots, head_dim / 32]");
   need(slots % 64 == 0 && slots <= (1 << 24), "a cache has a multiple of 64 slots, 2^24 at most");
   need(max_seq >= 0 && max_seq <= slots, "max_seq must be at most the cache's ", slots, " slots");
+  need(kc.size(1) >= 1, "a cache has at least one kv head");
   need(kc.size(0) <= 65535 && kc.size(1) <= 65535 && kc.size(1) * slots < (1ll << 30) &&
        kc.size(0) * kc.size(1) * (slots / 64) < (1ll << 30), "the cache has too many slots");
   need(kc.is_contiguous() && vc.is_contiguous() && ks.is_contiguous() && vs.is_contiguous(), "a cache's tensors must be contiguous");
@@ -1294,7 +1295,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     a.k = k.data_ptr();
     a.v = v.data_ptr();
     a.batch = (int)batch;
-    a.tokens = (int)k.size(1);
+    a.tokens = (int)std::min(k.size(1), max_seq);      // no more fit
     a.start = (int)start0;
     a.start_dev = int_ptr(start);
     a.counts = int_ptr(counts);

@@ -54,6 +54,11 @@ def test_cache_refuses_odd_slots_and_shared_memory():
     refused("share memory", ops.Kv4Cache, **p)
 
 
+def test_cache_refuses_no_heads():
+    none = {name: t[:, :0] for name, t in parts(weights=True).items()}
+    refused("at least one kv head", ops.Kv4Cache, **none)
+
+
 def test_new_refuses():
     for bad in (dict(head_dim=96), dict(max_seq=0), dict(n_kv_heads=0), dict(batch=-1)):
         refused("need|head_dim", ops.Kv4Cache.new, **{**dict(batch=1, max_seq=4, n_kv_heads=1, head_dim=64, device="cpu"), **bad})
