@@ -175,7 +175,7 @@ struct Attend {
     // 2^(120 - e): the largest element comes to [2^120, 2^121); e is held in [-6, 127], where the factor is a normal number
     const int e = min(max((int)(__float_as_uint(largest) >> 23) - 127, -6), 127);
     const float up = __uint_as_float((uint32_t)(120 - e + 127) << 23);
-    // S = 2^-133 n 2^(120 - e) q: back by 2^(13 + e), then log2(e) / sqrt(D)
+    // S = 2^-133 n 2^(120 - e) q: back by 2^(13 + e), then log2(e) / sqrt(D); an infinity from e = 118 on, the head's outputs NaN
     const float back = ldexpf(kLog2e * rsqrtf((float)D), 13 + e);
 #pragma unroll
     for (int j = 0; j < 2; ++j) to_log2[j] = __shfl_sync(0xffffffffu, back, 4 * (2 * c + j));

@@ -559,7 +559,8 @@ def new_kv4_caches(layers, batch: int, max_seq: int, track_weights: bool = False
 class Kv4Sequences:
     """A batch of sequences over 4-bit caches: what `LlamaTPStack` keeps of them with `kv_bits=4`.  `lengths` (slots in
     use) and `positions` (tokens seen), int32 [batch] on the GPU, advance with every step; with `use_graph` the step is
-    one captured CUDA graph.  A sequence is made idle by a negative length."""
+    one captured CUDA graph.  A sequence is made idle by a negative length; one that has filled its caches is idle too until
+    `evict` makes room (neither of its counts goes on)."""
 
     def __init__(self, layers, batch: int, max_seq: int, track_weights: bool = False, use_graph: bool = True):
         self.layers, self.max_seq = list(layers), int(max_seq)
@@ -585,7 +586,7 @@ class Kv4Sequences:
 
     def _run(self, x: torch.Tensor) -> torch.Tensor:
         y = decode_kv4_through(self.layers, self.caches, x, self.lengths, self.positions)
-        active = self.lengths >= 0
+        active = (self.lengths >= 0) & (self.lengths < self.max_seq)
         self.lengths += active
         self.positions += active
         return y

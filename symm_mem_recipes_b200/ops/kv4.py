@@ -114,7 +114,8 @@ def kv4_decode_attention_(qkv: torch.Tensor, cache: Kv4Cache, n_q_heads: int, le
 
     `lengths`: an int32 tensor [batch], or an int for all.  A sequence whose length is negative, or `max_seq` and more, is
     idle: its output row is zero and its cache is left alone.  `head_dim` is 64 or 128, hq / hkv at most 8, batch at most
-    1024.  A NaN or an infinity in a row of q, K or V shows in the outputs and weights that read it, and in no others."""
+    1024.  A NaN or an infinity in a row of q, K or V shows in the outputs and weights that read it, and in no others; a query
+    with a magnitude of 2^118 or more counts as one."""
     on_device = isinstance(lengths, torch.Tensor)
     return C.kv4_decode_attention(qkv, cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales, cache.weights,
                                   cache.max_seq, n_q_heads, 0 if on_device else lengths, lengths if on_device else None, out)

@@ -224,6 +224,17 @@ def test_append_outside_is_skipped():
     assert same(cache, want)
 
 
+def test_append_more_tokens_than_an_int_counts():
+    """One row, broadcast over 2^31 + 3 tokens: what fits is written, the rest dropped."""
+    cache = filled(16, 1, 70, 1, 64)
+    want = copy_of(cache)
+    k, v = normal(17, 1, 1, 1, 64), normal(18, 1, 1, 1, 64)
+    for t in range(66, 70):
+        put(want, 0, t, k[0, 0], v[0, 0])
+    ops.kv4_append_(k.expand(1, 2 ** 31 + 3, 1, 64), v.expand(1, 2 ** 31 + 3, 1, 64), cache, int32([66]))
+    assert same(cache, want)
+
+
 # ---- attention ----
 
 def check_attention(cache, qkv, hq, lengths, out, before):
@@ -322,6 +333,26 @@ def test_decode_attention_zero_values():
     assert not out.any()
     assert cache.weights[0, 0, 0].item() == 4.0
     assert bool(((cache.weights[1, 0, :71] - 4 / 71).abs() <= 2.0 ** -20).all()) and not cache.weights[1, 0, 71:].any()
+
+
+def test_decode_attention_large_queries():
+    """A query of 2^117 is a number, over keys of zero the mean of the values; one of 2^118 counts as an infinity."""
+    cache = filled(31, 1, 100, 1, 64)
+    cache.k_scales.zero_()
+    before = copy_of(cache)
+    qkv = normal(32, 1, 6 * 64)
+    qkv[0, 4 * 64:5 * 64] = 0
+    qkv[0, 64 + 5] = 2.0 ** 117
+    qkv[0, 2 * 64 + 5] = -2.0 ** 118
+    out = ops.kv4_decode_attention_(qkv, cache, 4, int32([90])).view(4, 64)
+    assert torch.isnan(out[2]).all() and int(torch.isnan(out).sum()) == 64
+    calm = normal(32, 1, 6 * 64)
+    calm[0, 4 * 64:5 * 64] = 0
+    cache = copy_of(before)
+    want = ops.kv4_decode_attention_(calm, cache, 4, int32([90]))
+    check_attention(cache, calm, 4, [90], want, before)
+    want = want.view(4, 64)
+    assert torch.equal(out[[0, 1, 3]], want[[0, 1, 3]])      # all scores are zero either way
 
 
 def test_decode_attention_nan_stays_where_it_is():
@@ -637,6 +668,22 @@ def test_stack_with_a_4_bit_cache():
     graph.reset()
     assert not graph.caches[0].weights.any() and graph.sequences.lengths.tolist() == [0] * 3
     assert len(new_kv_caches(plain.layers, 1, 4)) == 2
+
+
+def test_stack_of_full_caches():
+    """A sequence that has filled its caches waits, unchanged, until they are cut."""
+    stack = stack_of(kv_bits=4, track_weights=True)
+    stack.prefill(normal(91, 3 * 90, 512, std=0.5), 90)
+    stack.sequences.lengths[1] = stack.sequences.positions[1] = 95
+    for step in range(3):
+        stack.decode_step(normal(92 + step, 3, 512, std=0.5))
+    assert stack.sequences.lengths.tolist() == [93, 96, 93] and stack.sequences.positions.tolist() == [93, 96, 93]
+    stack.evict(40, recent=8)
+    before = [copy_of(c) for c in stack.caches]
+    stack.decode_step(normal(95, 3, 512, std=0.5))
+    assert stack.sequences.lengths.tolist() == [41] * 3 and stack.sequences.positions.tolist() == [94, 97, 94]
+    for was, now in zip(before, stack.caches):
+        assert not torch.equal(was.k_codes[1, :, 40], now.k_codes[1, :, 40])
 
 
 def test_stack_refuses():
