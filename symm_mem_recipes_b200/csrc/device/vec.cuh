@@ -27,7 +27,8 @@ __device__ __forceinline__ Vec16 ld_16_stream(const void* p) {
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
   return v;
 }
-// Read-only path for data that no one writes during the kernel (weights).
+// Read-only path for data that no one writes during the kernel (weights).  A kernel that starts under its predecessor
+// (pdl.cuh) takes what that one writes by the loads above, behind its pdl_wait too.
 __device__ __forceinline__ Vec16 ld_16_nc(const void* p) {
   Vec16 v;
   asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"

@@ -160,7 +160,7 @@ struct Attend {
                                ((size_t)h * a.group + r) * D + 8 * c;
     Vec16 raw[kG];
 #pragma unroll
-    for (int g = 0; g < kG; ++g) raw[g] = r < a.group ? ld_16_nc(row + kGroup * g) : Vec16{0, 0, 0, 0};
+    for (int g = 0; g < kG; ++g) raw[g] = r < a.group ? ld_16_stream(row + kGroup * g) : Vec16{0, 0, 0, 0};
     float largest = 0.0f;
 #pragma unroll
     for (int g = 0; g < kG; ++g) {

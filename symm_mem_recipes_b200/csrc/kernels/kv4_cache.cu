@@ -71,7 +71,7 @@ __device__ __forceinline__ void append_rows(const Kv4AppendArgs& a, const Diviso
 #pragma unroll
   for (int u = 0; u < kRows; ++u, row.next(hkv)) {
     raw[u] = Vec16{0, 0, 0, 0};
-    if (row.t < tokens) raw[u] = ld_16_nc(src + row.t * stride[1] + row.h * stride[2]);
+    if (row.t < tokens) raw[u] = ld_16_stream(src + row.t * stride[1] + row.h * stride[2]);
   }
   row = Row(first, hkv);
   const size_t base = (size_t)b * hkv.d * a.cache.slots + max(start, 0);

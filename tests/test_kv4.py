@@ -181,3 +181,27 @@ def test_cut_heads_are_joined_whole():
         rng = random.Random(seed)
         heads = [rng.choice((0, 1, 1, 2, 3, rng.randint(1, 40))) for _ in range(rng.randint(1, 14))]
         assert C.check_kv4_cuts(heads, rng.randint(1, 7)) == 0, (seed, heads)
+
+
+def kernels_of(name):
+    """(name, body) of the __global__ functions of a kernel file, comments taken out."""
+    import pathlib
+    import re
+    root = pathlib.Path(ops.__file__).resolve().parent.parent / "csrc" / "kernels"
+    text = re.sub(r"//[^\n]*", "", (root / name).read_text())
+    out = []
+    for m in re.finditer(r"__global__[^;{]*?(\w+)\((?:const\b|int\b|\w+\s+\w+)[^{;]*\)\s*\{", text):
+        depth, end = 1, m.end()
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        out.append((m.group(1), text[m.end():end]))
+    return text, out
+
+
+@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_cache.cu", "rope_axes.cu"])
+def test_inputs_are_loaded_coherently(name):
+    """The kernels start under the one in front, which may still write their inputs: no load by the read-only path."""
+    text, kernels = kernels_of(name)
+    assert len(kernels) >= 1 and all("pdl_wait()" in body for _, body in kernels)
+    assert "ld_16_nc" not in text and "ld.global.nc" not in text and "__ldg" not in text and "__restrict__" not in text
