@@ -64,14 +64,17 @@ struct Layout {
 struct Workspace {
   float* pieces;      // [warps][2][kPiece]: a warp's first head and its last one, where they are shared with others
   float2* stats;      // [batch * hkv][kHeads]
+  int* start;         // [batch + 1]: first tile of a sequence
   float* scores;      // [tiles][kTile][padded group], units of log2
 };
 __host__ __device__ inline int padded_group(int group) { return (group + 1) & ~1; }
-__host__ __device__ inline Workspace carve(void* base, int head_dim, int batch_heads, int warps) {
+__host__ __device__ inline int padded_starts(int batch) { return (batch + 2) & ~1; }
+__host__ __device__ inline Workspace carve(void* base, int head_dim, int batch, int hkv, int warps) {
   Workspace w;
   w.pieces = static_cast<float*>(base);
   w.stats = reinterpret_cast<float2*>(w.pieces + (size_t)warps * 2 * kHeads * (head_dim + 2));
-  w.scores = reinterpret_cast<float*>(w.stats + (size_t)batch_heads * kHeads);
+  w.start = reinterpret_cast<int*>(w.stats + (size_t)batch * hkv * kHeads);
+  w.scores = reinterpret_cast<float*>(w.start + padded_starts(batch));
   return w;
 }
 
@@ -504,12 +507,15 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
     if (lane >= o) before += y;
   }
   const int tiles = __shfl_sync(0xffffffffu, before, 31);
-  if (tiles == 0) return;      // every CTA
   before -= mine;
   const int warps = gridDim.x * kWarps, w = blockIdx.x * kWarps + warp;
+  const Workspace ws = carve(a.workspace, D, a.batch, hkv, warps);
+  if (tiles == 0) {      // every CTA
+    for (int i = threadIdx.x; blockIdx.x == 0 && i <= a.batch; i += 32 * kWarps) ws.start[i] = 0;
+    return;
+  }
   const Shares shares(tiles, warps);
   const int first = shares.first(w), end = shares.first(w + 1);
-  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
   Cursor now{0, 0, 0, 1};
   if (first < end) {
     int left = first - before;      // of the sequence that `first` is in, in the lane that has it
@@ -544,9 +550,13 @@ __global__ void __launch_bounds__(32 * kWarps, 2) attend_kernel(const __grid_con
   if (warp == 0) {
     for (int i = 0; i < per && b0 + i < a.batch; ++i) {
       start[b0 + i] = before;
+      if (blockIdx.x == 0) ws.start[b0 + i] = before;      // for the second kernel
       before += tiles_of(a, b0 + i) * hkv;
     }
-    if (lane == 31) start[a.batch] = tiles;
+    if (lane == 31) {
+      start[a.batch] = tiles;
+      if (blockIdx.x == 0) ws.start[a.batch] = tiles;
+    }
   }
   __syncthreads();
   auto advance = [&](Cursor& at) {
@@ -678,51 +688,27 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
                                                             int chunks) {
   using L = Layout<D>;
   constexpr int kJoinWarps = kJoinThreads / 32, kSide = D / 4, kLanes = 32 / kSide;      // kLanes pieces side by side in a warp
-  __shared__ int sums[2][kJoinWarps];
   __shared__ float norms[2][kHeads];
   __shared__ float part[kJoinWarps][2];
   __shared__ float4 parts[kJoinWarps][kSide];
   const int bh = blockIdx.x, hkv = a.cache.hkv, b = bh / hkv, h = bh % hkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // The lengths are no output of the first kernel: it has waited for what wrote them before it let this one start.
-  const int n = tiles_of(a, b);
+  pdl_launch_dependents();
+  pdl_wait();
+  const Workspace ws = carve(a.workspace, D, a.batch, hkv, warps);
+  // three loads side by side; the lengths too belong to the kernels in front, and are nobody's to read before the wait
+  const int n = tiles_of(a, b), first = ws.start[b], all = ws.start[a.batch];
+  const int chunk0 = (int)blockIdx.y - outputs;
   if (n == 0) {      // idle: the output row is zero
-    pdl_wait();
     if (blockIdx.y == 0)
       for (int i = tid; i < a.group * D / 8; i += kJoinThreads)
         st_16(static_cast<__nv_bfloat16*>(a.out) + (size_t)bh * a.group * D + i * 8, Vec16{0, 0, 0, 0});
     return;
   }
-  const int chunk0 = (int)blockIdx.y - outputs;
   if (kScores && chunk0 >= 0 && chunk0 * kJoinTiles >= n) return;
-  int before = 0, all = 0;
-  for (int i = tid; i < a.batch; i += kJoinThreads) {
-    const int t = tiles_of(a, i);
-    all += t;
-    before += i < b ? t : 0;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-  }
-  if (lane == 0) {
-    sums[0][warp] = before;
-    sums[1][warp] = all;
-  }
-  __syncthreads();
-  before = all = 0;
-#pragma unroll
-  for (int i = 0; i < kJoinWarps; ++i) {
-    before += sums[0][i];
-    all += sums[1][i];
-  }
-  const Workspace ws = carve(a.workspace, D, a.batch * hkv, warps);
-  const int s0 = before * hkv + h * n;
-  pdl_launch_dependents();
-  const HeadCut cut(Shares(all * hkv, warps), s0, s0 + n);
+  const int s0 = first + h * n;
+  const HeadCut cut(Shares(all, warps), s0, s0 + n);
   auto piece = [&](int k) -> const float* { return ws.pieces + (size_t)cut.place(k) * L::kPiece; };
 
-  pdl_wait();
   if (chunk0 < 0) {
     if (cut.finished) return;
     // kJoinWarps / per warps a query head, each every `sides`-th group of pieces; four dims a thread
@@ -1081,7 +1067,8 @@ int launch(const Kv4AttentionArgs& a, cudaStream_t stream) {
 size_t kv4_attention_workspace_bytes(const Kv4Cache& cache, int batch, int group, int num_sms) {
   if (head_ctas(cache, batch, num_sms) > 0) return 0;
   const size_t warps = (size_t)attention_ctas(cache, batch, num_sms) * kWarps;
-  size_t bytes = warps * 2 * kHeads * (cache.head_dim + 2) * sizeof(float) + (size_t)batch * cache.hkv * kHeads * sizeof(float2);
+  size_t bytes = warps * 2 * kHeads * (cache.head_dim + 2) * sizeof(float) + (size_t)batch * cache.hkv * kHeads * sizeof(float2) +
+                 padded_starts(batch) * sizeof(int);
   if (cache.weights != nullptr) bytes += (size_t)batch * cache.hkv * cache.slots * padded_group(group) * sizeof(float);
   return bytes;
 }

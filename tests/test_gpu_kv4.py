@@ -615,6 +615,36 @@ def test_steps_back_to_back_are_the_steps_one_by_one(batch, hkv, max_seq):
     assert torch.equal(results[0][0], results[1][0]) and same(results[0][1], results[1][1])
 
 
+@pytest.mark.parametrize("batch, hkv, max_seq", [(9, 8, 9000), (2, 4, 21000)])
+def test_evict_then_decode_with_nothing_between(batch, hkv, max_seq):
+    """Lengths that an eviction has just written, straight into a decode step of two launches, five times over: the bits of
+    the same calls with pauses."""
+    g, dim = 5, 128
+    xs = [normal(101 + i, batch, (g + 2) * hkv * dim) for i in range(5)]
+    full = torch.randint(max_seq - 200, max_seq + 1, (batch,), generator=gen(100), device="cuda").int()
+    full[0] = -1
+    if batch > 2:
+        full[1] = 17
+    results = []
+    for pause in (True, False):
+        cache = filled(102, batch, max_seq, hkv, dim, weights=True)
+        lengths, outs, news = full.clone(), [], []
+        torch.cuda.synchronize()
+        for i, x in enumerate(xs):
+            lengths = ops.kv4_evict_(cache, lengths, max_seq - 300 - 1500 * i, recent=5)
+            if pause:
+                torch.cuda.synchronize()
+            outs.append(ops.kv4_decode_attention_(x, cache, g * hkv, lengths))
+            news.append(lengths)
+            if pause:
+                torch.cuda.synchronize()
+        results.append((torch.stack(outs), torch.stack(news), cache))
+    torch.cuda.synchronize()
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    assert same(results[0][2], results[1][2])
+    assert results[0][1][-1].max().item() == max_seq - 6300
+
+
 # ---- the layer and the stack ----
 
 def stack_of(**kw):

@@ -205,3 +205,13 @@ def test_inputs_are_loaded_coherently(name):
     text, kernels = kernels_of(name)
     assert len(kernels) >= 1 and all("pdl_wait()" in body for _, body in kernels)
     assert "ld_16_nc" not in text and "ld.global.nc" not in text and "__ldg" not in text and "__restrict__" not in text
+
+
+@pytest.mark.parametrize("name", ["kv4_attention.cu", "kv4_cache.cu", "rope_axes.cu"])
+def test_nothing_is_read_before_the_wait(name):
+    """Lengths, positions and caches belong to the kernels in front until pdl_wait has returned, and every CTA calls it: what
+    stands in front of it uses the launch's arguments alone."""
+    for kernel, body in kernels_of(name)[1]:
+        before = body[:body.index("pdl_wait()")]
+        for word in ("tiles_of", "length_of", "lengths[", "pos[", "positions[", "ld_16", "return", "ws."):
+            assert word not in before, (kernel, word)
