@@ -559,8 +559,9 @@ def new_kv4_caches(layers, batch: int, max_seq: int, track_weights: bool = False
 class Kv4Sequences:
     """A batch of sequences over 4-bit caches: what `LlamaTPStack` keeps of them with `kv_bits=4`.  `lengths` (slots in
     use) and `positions` (tokens seen), int32 [batch] on the GPU, advance with every step; with `use_graph` the step is
-    one captured CUDA graph.  A sequence is made idle by a negative length; one that has filled its caches is idle too until
-    `evict` makes room (neither of its counts goes on)."""
+    one captured CUDA graph.  A sequence is made idle by a negative length (who means to go on with it keeps its length and writes
+    that back); one that has filled its caches, `lengths[b] >= max_seq`, is idle too until `evict` makes room (neither of its counts
+    goes on)."""
 
     def __init__(self, layers, batch: int, max_seq: int, track_weights: bool = False, use_graph: bool = True):
         self.layers, self.max_seq = list(layers), int(max_seq)
@@ -696,7 +697,8 @@ class LlamaTPStack:
 
     With `kv_bits=4` the caches hold 4.5 bits a value (`stack.sequences`, a `Kv4Sequences`, has them with the sequences'
     lengths and positions); with `track_weights` too, `stack.evict(keep, recent)` cuts them to the heaviest slots between two
-    steps.  `pos` is then the number of tokens before this one for all sequences, or None to go on from `sequences.positions`.
+    steps.  `pos` is then the number of tokens before this one for all sequences, or None to go on from `sequences.positions`; the
+    slot is the next one either way (`decode_step` has the differences).
     """
 
     def __init__(self, cfg: LlamaTPConfig, n_layers: int, device: torch.device, batch: int, max_seq: int,
@@ -749,9 +751,17 @@ class LlamaTPStack:
 
     def decode_step(self, x: torch.Tensor, pos: Optional[int] = None) -> torch.Tensor:
         """One token per sequence at position `pos`: [batch, H] in (replicated), [batch, H] out.  With
-        the graph the result tensor is overwritten by the next step."""
+        the graph the result tensor is overwritten by the next step.
+
+        Over 4-bit caches `pos` turns queries and keys and no more: the token goes into slot `sequences.lengths[b]`, so that a
+        step at an earlier `pos` adds a token where one over 16-bit caches replaces it (set `sequences.lengths` back for
+        that), and `pos` may pass `max_seq` once caches were cut.  A sequence whose caches are full
+        (`sequences.lengths[b] >= max_seq`) is idle: its token is not kept and sees nothing, without an error, because the
+        lengths are the GPU's; a loop that may fill its caches looks at them or cuts them in time."""
         if self.sequences is not None:
             if pos is not None:
+                if not 0 <= pos < 2 ** 31:
+                    raise ValueError(f"position {pos} is not an int32 position")
                 self.sequences.positions.fill_(pos)
             return self.sequences.step(x)
         if pos is None:

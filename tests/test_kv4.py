@@ -183,6 +183,26 @@ def test_cut_heads_are_joined_whole():
         assert C.check_kv4_cuts(heads, rng.randint(1, 7)) == 0, (seed, heads)
 
 
+def test_stack_refuses_positions_that_are_none():
+    """A step over 4-bit caches takes positions of 32 bits; refused before anything is written."""
+    from symm_mem_recipes_b200.models.llama_tp_layer import LlamaTPStack
+
+    class Sequences:
+        positions = torch.full((3,), 7, dtype=torch.int32)
+
+        def step(self, x):
+            return x + 1
+
+    stack = LlamaTPStack.__new__(LlamaTPStack)
+    stack.sequences = Sequences()
+    for pos in (-1, 2 ** 31, 2 ** 31 + 5, -2 ** 40):
+        with pytest.raises(ValueError, match="position"):
+            stack.decode_step(torch.zeros(1), pos)
+    assert stack.sequences.positions.tolist() == [7] * 3
+    assert stack.decode_step(torch.zeros(1), 2 ** 31 - 1).item() == 1 and stack.sequences.positions.tolist() == [2 ** 31 - 1] * 3
+    assert stack.decode_step(torch.zeros(1)).item() == 1
+
+
 def kernels_of(name):
     """(name, body) of the __global__ functions of a kernel file, comments taken out."""
     import pathlib
