@@ -43,6 +43,7 @@ from __future__ import annotations
 
 import contextlib
 import os
+import warnings
 from dataclasses import dataclass
 from typing import Optional
 
@@ -571,6 +572,7 @@ class Kv4Sequences:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.positions = torch.zeros(batch, dtype=torch.int32, device=dev)
         self.graph = None
+        self._weighed = True      # a step has run since the last prompt: its attention weighed the slots
         if use_graph:
             self.x = torch.zeros(batch, first.cfg.hidden, dtype=torch.bfloat16, device=dev)
             # first calls allocate workspaces and rendezvous: outside the capture, on a side stream
@@ -596,16 +598,19 @@ class Kv4Sequences:
         """Start new sequences."""
         for cache in self.caches:
             cache.reset()
+        self._weighed = True
         self.lengths.zero_()
         self.positions.zero_()
 
     def begin(self, seq: int) -> None:
         """A prompt of `seq` tokens is in the caches."""
+        self._weighed = False
         self.lengths.fill_(seq)
         self.positions.fill_(seq)
 
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """The next token of every sequence: [batch, H] in and out; with the graph the result is overwritten by the next step."""
+        self._weighed = True
         if self.graph is None:
             return self._run(x)
         self.x.copy_(x)
@@ -613,7 +618,12 @@ class Kv4Sequences:
         return self.y
 
     def evict(self, keep: int, recent: int = 0) -> None:
-        """Cut every layer's caches to `keep` slots a sequence (`ops.kv4_evict_`); positions go on counting tokens."""
+        """Cut every layer's caches to `keep` slots a sequence (`ops.kv4_evict_`); positions go on counting tokens.  Only steps weigh
+        slots, a prompt's own attention does not: right after a prompt all weights are equal, and besides the `recent` slots
+        the oldest would stay.  That call warns; a few steps in between, or `recent=keep` for the newest slots, is meant."""
+        if recent < keep and not self._weighed:
+            warnings.warn("evict: no step since the prompt has weighed its slots, so besides the recent ones the oldest stay",
+                          stacklevel=2)
         for cache in self.caches:
             lengths = ops.kv4_evict_(cache, self.lengths, keep, recent)
         self.lengths.copy_(lengths)
@@ -744,7 +754,8 @@ class LlamaTPStack:
         return h
 
     def evict(self, keep: int, recent: int = 0) -> None:
-        """Cut 4-bit caches that track weights to `keep` slots a sequence, between two steps."""
+        """Cut 4-bit caches that track weights to `keep` slots a sequence, between two steps (`Kv4Sequences.evict`: after a
+        prompt only once steps have weighed its slots)."""
         if self.sequences is None:
             raise ValueError("eviction needs kv_bits=4 and track_weights")
         self.sequences.evict(keep, recent)

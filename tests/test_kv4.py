@@ -203,6 +203,31 @@ def test_stack_refuses_positions_that_are_none():
     assert stack.decode_step(torch.zeros(1)).item() == 1
 
 
+def test_eviction_right_after_a_prompt_warns(monkeypatch):
+    """No step has weighed the prompt's slots: all but the recent ones would stay by their age."""
+    import warnings
+
+    from symm_mem_recipes_b200.models.llama_tp_layer import Kv4Sequences
+    cuts = []
+    monkeypatch.setattr(ops, "kv4_evict_", lambda cache, lengths, keep, recent: cuts.append((cache, keep, recent)) or lengths.clamp(max=keep))
+    seq = Kv4Sequences.__new__(Kv4Sequences)
+    seq.caches, seq.graph, seq.lengths, seq.positions = ["a", "b"], None, torch.zeros(2, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    seq._run = lambda x: x
+    seq.begin(50)
+    with pytest.warns(UserWarning, match="no step since the prompt"):
+        seq.evict(30, recent=4)
+    assert cuts == [("a", 30, 4), ("b", 30, 4)] and seq.lengths.tolist() == [30, 30] and seq.positions.tolist() == [50, 50]
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        seq.evict(20, recent=20)
+        seq.step(torch.zeros(1))
+        seq.evict(10)
+        seq.begin(60)
+        seq.step(torch.zeros(1))
+        seq.evict(10, recent=3)
+    assert seq.lengths.tolist() == [10, 10]
+
+
 def kernels_of(name):
     """(name, body) of the __global__ functions of a kernel file, comments taken out."""
     import pathlib
