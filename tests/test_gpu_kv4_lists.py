@@ -132,3 +132,25 @@ def test_long_lists_in_graphs_side_by_side():
     torch.cuda.synchronize()
     for (o, c), got, cache in zip(want, outs, caches):
         assert torch.equal(o, got) and same(c, cache)
+
+
+@pytest.mark.parametrize("weights", [False, True])
+def test_a_list_without_tiles(weights):
+    """All sequences idle, in the form of two launches: rows of zeros, nothing else touched; then one of them goes on."""
+    batch, hkv, g, dim = 80, 8, 2, 128
+    cache = filled(230, batch, 128, hkv, dim, weights)
+    before = copy_of(cache)
+    qkv = normal(231, batch, (g + 2) * hkv * dim)
+    lengths = [(-1, 128, -2 ** 31, 2 ** 31 - 1)[b % 4] for b in range(batch)]
+    out = torch.full((batch, g * hkv * dim), 3.0, dtype=torch.bfloat16, device="cuda")
+    assert not ops.kv4_decode_attention_(qkv, cache, g * hkv, int32(lengths), out=out).any() and same(cache, before)
+    lengths[77] = 0
+    out = ops.kv4_decode_attention_(qkv, cache, g * hkv, int32(lengths))
+    put(before, 77, 0, *(qkv[77].view(-1, hkv, dim)[i] for i in (g, g + 1)))
+    if weights:
+        before.weights[77, :, 0] = g
+    v = ref.values(ref.unpack(before.v_codes[77, :, 0], False), before.v_scales[77, :, 0]).repeat_interleave(g, dim=0)
+    assert not out[:77].any() and not out[78:].any() and same(cache, before)
+    # one slot of probability 1: the scale in fp16 (8 bits of 11, exact), sums cut at 2^-10.9 s and 2^-18.4 15 s, the result in bf16
+    tol = 2.0 ** -8 * v.abs() + (2.0 ** -10.9 + 4 * 2.0 ** -18.4) * before.v_scales[77, :, 0].double().repeat_interleave(32, dim=1).repeat_interleave(g, dim=0)
+    assert bool(((out[77].view(hkv * g, dim).double() - v).abs() <= tol).all())
