@@ -19,12 +19,13 @@
 //   near 2^120; a group's 32 dims are two MMAs, whose sum the key's scale multiplies in fp32.  No operand is rounded.
 //   O^T [16 dims x 8 heads] += V^T P'^T, fp16: P' = 2^(S - M) * scale, where the values' scale of the key and group goes
 //   into the probability.  M is at least (largest S of a tile) + (exponent of its largest scale) - 15, so P' stays below
-//   2^15 and is rounded to 11 bits (2^-12 of itself) down to 2^-29 of the largest; the output is rounded to 8 bits.
+//   2^15 and is rounded to 11 bits (2^-11 of itself) down to 2^-29 of the largest; the output is rounded to 8 bits.
 // S^T's accumulators hold heads in rows of four lanes, the second MMA wants keys there: movmatrix transposes in registers.
 //
-// Measured: 1.67 us per 1000 tiles at D = 128 (5.5 TB/s, 84 % of the copy rate) and 16 us besides; 32 x 8 heads of 6600 to 16384 slots
-// 103 us, 8 heads of 131072 with weights 53.  Reading alone takes 72 of the 103, computing alone 80: neither memory nor one
-// pipe is full (issue 52 %, ALU 51 %, tensor 32 %).  Three CTAs an SM, bulk copies and one stage less are no faster.
+// Measured: 1.67 us per 1000 tiles at D = 128 (5.5 TB/s, 84 % of the copy rate) and 18 us besides; 32 x 8 heads of 6600 to 16384 slots
+// (46592 tiles) 96 us in bursts and 103 in a long loop, where the 1000 W cap lowers the clock; 8 heads of 131072 with weights 53.
+// Reading alone takes 72, computing alone 80: neither memory nor one pipe is full (issue 52 %, ALU 51 %, tensor 32 %).  Three CTAs
+// an SM, bulk copies and one stage less are no faster.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -1,9 +1,11 @@
 // Rotary embedding in place, with a position of its own for every token and axis (time, row, column of images and video).
 //
 // Pair i of a head, (x_i, x_{i + D/2}), turns by pos[axis(i)] * theta^(-2i / D); the frequencies run over the whole head
-// and the axis only chooses whose position a pair sees.  Angles are kept as turns in 64-bit fixed point: frequency
+// and the axis only chooses whose position a pair sees.  Angles are reduced as turns in 64-bit fixed point: frequency
 // theta^(-2i / D) / (2 pi) times 2^64, rounded, times the integer position, modulo 2^64, is the angle's fraction of a turn
-// to 2^-33 for every 32-bit position, where an fp32 product has lost 0.01 rad at position 200000.
+// to 2^-34 for every 32-bit position, where an fp32 product has lost 0.01 rad at position 200000.  Of it the upper 32 bits are
+// used (2^-32 of a turn), turned into an fp32 angle, at most 2^-21.3 off; the sine and cosine intrinsics add 2^-21.1: 2^-20 of
+// |x| + |y|, where the result is rounded to 2^-8 of itself.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -33,9 +35,9 @@ __device__ __forceinline__ Vec16 pack8(const float (&f)[8]) {
 }
 
 // A CTA takes `per` tokens: first the (cos, sin) of their D / 2 pairs, then the heads, eight pairs a thread and step.  Bound by
-// HBM: 8192 tokens of 72 heads of 128 (302 MB read and written) 51.0 us, 91 % of the copy rate; several steps' loads in
-// flight at a time were slower (two 52, four 66).  kOnce: the result is more than L2 keeps, its lines are the first to
-// leave (53.3 us without).
+// HBM: 8192 tokens of 72 heads of 128 (302 MB read and written) 58.5 us, 79 % of the copy rate; several steps' loads in
+// flight at a time were slower (two by 2 %, four by 29 %).  kOnce: the result is more than L2 keeps, its lines are the first to
+// leave (61.0 us without).
 template <int D, bool kOnce>
 __global__ void __launch_bounds__(kThreads) rope_axes_kernel(const __grid_constant__ RopeAxesArgs a, int per) {
   constexpr int kPairs = D / 2, kVecs = D / 16;

@@ -115,7 +115,11 @@ def kv4_decode_attention_(qkv: torch.Tensor, cache: Kv4Cache, n_q_heads: int, le
     `lengths`: an int32 tensor [batch], or an int for all.  A sequence whose length is negative, or `max_seq` and more, is
     idle: its output row is zero and its cache is left alone.  `head_dim` is 64 or 128, hq / hkv at most 8, batch at most
     1024.  A NaN or an infinity in a row of q, K or V shows in the outputs and weights that read it, and in no others; a query
-    with a magnitude of 2^118 or more counts as one."""
+    with a magnitude of 2^118 or more counts as one, and so does a score beyond fp32.
+
+    Scores, maxima, sums and weights are fp32.  A probability times the scale of a value's group is rounded to fp16 on its way into
+    the weighted sum: 2^-11 of itself at most while it is at least 2^-29 of the largest probability times the largest scale in 64
+    slots, for values between 2^-56 and 2^100.  Smaller products lose bits, and below 2^-40 they count as zero."""
     on_device = isinstance(lengths, torch.Tensor)
     return C.kv4_decode_attention(qkv, cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales, cache.weights,
                                   cache.max_seq, n_q_heads, 0 if on_device else lengths, lengths if on_device else None, out)

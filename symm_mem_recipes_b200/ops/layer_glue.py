@@ -88,8 +88,8 @@ def rope_axes_(qkv: torch.Tensor, n_heads: int, head_dim: int, positions: torch.
     of a head, dims `(i, i + head_dim / 2)`, turns by `position * theta ** (-2 i / head_dim)` with the position of one axis:
     `sections` says how many of the head_dim / 2 pairs each axis has, the first axis the first pairs and so on, or with
     `interleaved` dealt in turn until an axis has its share.  For images and video the axes are time, row and column; for
-    text all positions of a token are equal, which is plain RoPE.  Angles are exact for every position (64-bit turns), sines
-    fp32, results rounded to bfloat16.  `inverse` rotates back, which is also the gradient of the rotation.  Rows may be
+    text all positions of a token are equal, which is plain RoPE.  Angles are reduced in 64-bit fixed point, so no position
+    loses bits; sine and cosine are within 2^-20 for all of them, results rounded to bfloat16.  `inverse` rotates back, which is also the gradient of the rotation.  Rows may be
     strided (on 16 bytes); head_dim is 64 or 128.  Positions are read when the kernel runs."""
     C.rope_axes(qkv, n_heads, head_dim, positions, sections, theta, interleaved, inverse)
     return qkv
