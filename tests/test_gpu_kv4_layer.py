@@ -131,3 +131,25 @@ def test_layer_over_a_4_bit_cache_world_of_one():
 @pytest.mark.multigpu(2)
 def test_layer_over_a_4_bit_cache_2gpu():
     spawn_ranks(_worker, 2, "nccl")
+
+
+def test_tensor_parallel_prefill_into_a_4_bit_cache():
+    """`forward_tp` leaves in a 4-bit cache what `kv4_append_` makes of its 16-bit keys and values."""
+    from symm_mem_recipes_b200 import ops
+    from symm_mem_recipes_b200.models.llama_tp_layer import LlamaTPConfig, LlamaTPDecoderLayer
+
+    dev = torch.device("cuda", 0)
+    torch.cuda.set_device(0)
+    cfg = LlamaTPConfig.tiny(1)
+    for fused_glue in (True, False):
+        layer = LlamaTPDecoderLayer(cfg, dev, seed=3, fused_glue=fused_glue)
+        x = (torch.randn(2 * 33, cfg.hidden, generator=torch.Generator().manual_seed(1)) * 0.5).to(torch.bfloat16).to(dev)
+        kv = tuple(torch.zeros(2, 33, layer.hkv, cfg.head_dim, dtype=torch.bfloat16, device=dev) for _ in range(2))
+        cache, want = (ops.Kv4Cache.new(2, 50, layer.hkv, cfg.head_dim, dev, track_weights=True) for _ in range(2))
+        y = layer.forward_tp(x, 2, 33, kv_cache=kv)
+        assert torch.equal(layer.forward_tp(x, 2, 33, kv_cache=cache), y)
+        ops.kv4_append_(*kv, want)
+        for name in ("k_codes", "k_scales", "v_codes", "v_scales", "weights"):
+            assert torch.equal(getattr(cache, name), getattr(want, name)), name
+        with pytest.raises(ValueError, match="Kv4Cache of this batch"):
+            layer.forward_tp(x, 2, 33, kv_cache=ops.Kv4Cache.new(2, 32, layer.hkv, cfg.head_dim, dev))
